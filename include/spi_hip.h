@@ -30,7 +30,7 @@ typedef void* spi_stream_t;           /* hipStream_t */
 #define SPI_ERR_UNSUPPORTED -2        /* valid request this build has no kernel for */
 #define SPI_ERR_LAUNCH      -3        /* hipGetLastError() != hipSuccess after the launch */
 
-#define SPI_ABI_VERSION 13   /* 2: spi_raymarch_bwd gained d_color_scale, spi_triplane_decode_bwd_sorted gained d_rgb_scale
+#define SPI_ABI_VERSION 14   /* 2: spi_raymarch_bwd gained d_color_scale, spi_triplane_decode_bwd_sorted gained d_rgb_scale
                              * 3: spi_conv_desc gained workspace / workspace_bytes (Winograd path), spi_conv2d_workspace_bytes
                              * 4: + spi_sample_from_planes_fwd / _bwd (additive)
                              * 5: + contextual / roi_align / adam_pred / filtered_lrelu_fused   6: + spi_affine_fwd / _bwd   7: + spi_decoder_gains (additive)
@@ -41,7 +41,8 @@ typedef void* spi_stream_t;           /* hipStream_t */
                              *     + spi_upfirdn2d_fused_t / spi_tail_bwd_t / spi_chan_dot_t / spi_seg_flags_t / spi_filtered_lrelu_t,
                              *     SPI_DTYPE_F64 for spi_bias_act_t / spi_upfirdn2d_t (additive)
                              * 12: + spi_tail_bwd_dot_t (additive); spi_conv2d_workspace_bytes / workspace of fp16 activation tensors select the direct fp16 kernels
-                             * 13: + spi_conv_wino_f4_set (additive); the Winograd workspace of a >= 256^2 layer is 2.25x larger (36 instead of 16 frequencies) */
+                             * 13: + spi_conv_wino_f4_set (additive); the Winograd workspace of a >= 256^2 layer is 2.25x larger (36 instead of 16 frequencies)
+                             * 14: + spi_norm_residual_fwd / _bwd, spi_quantize_rows, spi_linear_int8, spi_grouped_linear_fwd / _dgrad / _wgrad, SPI_DTYPE_BF16 / _I8 (additive) */
 int         spi_abi_version(void);
 int         spi_sizeof_conv_desc(void);   /* sizeof(spi_conv_desc) of THIS build: bindings assert it against their own struct */
 const char* spi_last_error(void);     /* thread-local, valid until the next failing call */
@@ -241,7 +242,8 @@ int spi_upfirdn2d(const float* x, const float* f, float* y, int N, int C, int in
  * contract filtered_lrelu's rc = -1 has in the reference.
  * spi_upfirdn2d_t takes element strides {n, c, h, w} of x and y (NULL = dense NCHW): dense NCHW and channels_last are accepted, in any
  * combination, like the plugin's "non-overlapping and dense" rule (upfirdn2d.cpp:23).  No fused epilogue on this entry point. */
-enum { SPI_DTYPE_F32 = 0, SPI_DTYPE_F16 = 1, SPI_DTYPE_F64 = 2 };   /* F64: spi_bias_act_t / spi_upfirdn2d_t only (the plugins' double instantiation) */
+enum { SPI_DTYPE_F32 = 0, SPI_DTYPE_F16 = 1, SPI_DTYPE_F64 = 2,    /* F64: spi_bias_act_t / spi_upfirdn2d_t only (the plugins' double instantiation) */
+       SPI_DTYPE_BF16 = 3, SPI_DTYPE_I8 = 4 };                       /* the row operators (spi_norm_residual_*, spi_quantize_rows, spi_linear_int8, spi_grouped_linear_*) only */
 int spi_bias_act_t(const void* x, const void* b, const void* xref, const void* yref, const void* dy, void* y, int64_t n, int sizeB,
                    int64_t stepB, int grad, int act, float alpha, float gain, float clamp, int dtype, spi_stream_t stream);
 int spi_upfirdn2d_t(const void* x, const float* f, void* y, int N, int C, int inH, int inW, const int64_t* x_strides,
@@ -521,6 +523,95 @@ int spi_adam_multi_pred(void* const* ptrs, const int64_t* sizes, int T, int64_t 
  * each replay. */
 int spi_adam_multi_dev(void* const* ptrs, const int64_t* sizes, int T, int64_t max_size, const float* hyper,
                        float beta1, float beta2, float eps, spi_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Residual blocks of vectors (latent rows through fully connected layers): the norms around a block,
+ * products in 8-bit integers, products of ragged groups.  The reference has the plain pieces only:
+ * normalize_2nd_moment and FullyConnectedLayer, networks_stylegan2.py:27-29, 95-127.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* Norms before and after a block, fused with its gate and residual scale.  Rows h, residual [rows, width], contiguous, of type `dtype`:
+ *   z = Norm(h) * post_weight + post_bias  if `after`, else h;     s = residual + scale * a(gate) * z      -> stream_out (rounded once)
+ *   y = Norm(s) * pre_weight + pre_bias    if `before` (of the unrounded s)                               -> normed, or q / q_scale
+ *   Norm(x) = (x - m) / sqrt(mean((x - m)^2) + eps), m = mean(x) if `layer`, else 0;  a: SPI_ACT_LINEAR / _TANH / _SIGMOID
+ * gate_mode 0 none, 1 [width], 2 [rows / rows_per_sample, width], 3 [rows, width].  Weights, biases and gate: fp32 or `dtype`; biases may be NULL.
+ * q [rows, q_stride] with q_stride = width .. width rounded up to 16 (the padding is written as 0): q = rint(y / t), t = max|y| / 127 -> q_scale [rows].
+ * stats [rows, 4] (mean and 1/deviation of both norms): written by _fwd if not NULL, read by _bwd.  width <= SPI_NORM_MAX_WIDTH, _bwd _MAX_WIDTH_BWD.
+ * _bwd: d_stream (NULL = 0) and, if `before`, d_normed in; every other gradient pointer may be NULL (not wanted); weight and shared-gate gradients are sums
+ * over rows in a fixed order.  rows >= 1; workspace: spi_norm_residual_bwd_workspace(d) bytes. */
+#define SPI_NORM_MAX_WIDTH 32768
+#define SPI_NORM_MAX_WIDTH_BWD 8192
+typedef struct spi_norm_residual_desc {
+    int64_t rows, rows_per_sample;
+    int width, dtype, weight_dtype, gate_dtype, gate_mode, gate_act, layer, after, before;
+    float scale, eps;
+    const void *h, *residual, *gate, *post_weight, *post_bias, *pre_weight, *pre_bias;
+    void *stream_out, *normed;
+    int8_t* q;
+    float* q_scale;
+    int64_t q_stride;
+    float* stats;
+    const void *d_stream, *d_normed;
+    void *d_h, *d_residual, *d_gate, *d_post_weight, *d_post_bias, *d_pre_weight, *d_pre_bias;
+    void* workspace;
+    int64_t workspace_bytes;
+} spi_norm_residual_desc;
+int spi_sizeof_norm_residual_desc(void);
+int spi_norm_residual_fwd(const spi_norm_residual_desc* d, spi_stream_t stream);
+int64_t spi_norm_residual_bwd_workspace(const spi_norm_residual_desc* d);
+int spi_norm_residual_bwd(const spi_norm_residual_desc* d, spi_stream_t stream);
+
+/* Rows in 8 bits with a scale each: t = max|x| / 127 -> scale [rows] (fp32), q = clamp(rint(x / t), -127, 127) (IEEE division, ties to even; an all-zero row
+ * gives t = 0, q = 0; a row with an infinity or NaN t = NaN, q = 0).  x [rows, width] with rows x_stride elements apart, q rows q_stride bytes apart
+ * (width <= q_stride; the bytes up to min(q_stride, width rounded up to 16) are written as 0). */
+int spi_quantize_rows(const void* x, int64_t rows, int width, int64_t x_stride, int dtype, int8_t* q, int64_t q_stride, float* scale, spi_stream_t stream);
+
+/* y [M,N] = clamp(act(x_scale[m] * w_scale[n] * sum_k q[m,k] w[n,k] + bias[n]) * gain), the sum in 32-bit integers (exact: K <= SPI_LINEAR_INT8_MAX_K).
+ * x: int8 rows (x_dtype = SPI_DTYPE_I8, x_scale given), or rows of fp32 / fp16 / bf16, which the call quantises as spi_quantize_rows does.
+ * x rows x_stride elements, w rows w_stride bytes apart; y contiguous, of type y_dtype; bias fp32 or NULL; act: any SPI_ACT_*.
+ * w_bytes: bytes that may be read from w (>= (N-1) * w_stride + K).  workspace: spi_linear_int8_workspace(d) bytes. */
+#define SPI_LINEAR_INT8_MAX_K 131071
+typedef struct spi_linear_int8_desc {
+    int64_t M;
+    int N, K, x_dtype, y_dtype;
+    int64_t x_stride, w_stride, w_bytes;
+    const void* x;
+    const float* x_scale;
+    const int8_t* w;
+    const float *w_scale, *bias;
+    void* y;
+    int act;
+    float alpha, gain, clamp;
+    void* workspace;
+    int64_t workspace_bytes;
+} spi_linear_int8_desc;
+int spi_sizeof_linear_int8_desc(void);
+int64_t spi_linear_int8_workspace(const spi_linear_int8_desc* d);
+int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t stream);
+
+/* Products of ragged groups of rows: group e is the rows offsets[e] .. offsets[e+1]-1 of x [T,K] (offsets: E+1 int32 in DEVICE memory; read as their running
+ * maximum, clamped to 0 .. T).  Contiguous tensors of one type (fp32, fp16, bf16), sums in fp32:
+ *   _fwd:   y [T,N]     = gain * x W[e]^T + bias[e]      (W [E,N,K], bias [E,N] or NULL);  rows of no group: 0
+ *   _dgrad: dx [T,K]    = gain * dy W[e];                                                  rows of no group: 0
+ *   _wgrad: dw [E,N,K]  = gain * dy^T x over the group,  db [E,N] = column sums of dy;     either may be NULL; empty groups: 0
+ * workspace: spi_grouped_linear_workspace(d, pass) bytes (pass 0 forward, 1 dgrad, 2 wgrad). */
+typedef struct spi_grouped_linear_desc {
+    int64_t T;
+    int E, N, K, dtype;
+    float gain;
+    const void *x, *w, *bias;
+    const int32_t* offsets;
+    void* y;
+    const void* dy;
+    void *dx, *dw, *db;
+    void* workspace;
+    int64_t workspace_bytes;
+} spi_grouped_linear_desc;
+int spi_sizeof_grouped_linear_desc(void);
+int64_t spi_grouped_linear_workspace(const spi_grouped_linear_desc* d, int pass);
+int spi_grouped_linear_fwd(const spi_grouped_linear_desc* d, spi_stream_t stream);
+int spi_grouped_linear_dgrad(const spi_grouped_linear_desc* d, spi_stream_t stream);
+int spi_grouped_linear_wgrad(const spi_grouped_linear_desc* d, spi_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -4,6 +4,7 @@ Thin by design: tensors go down as raw device pointers + sizes + the current HIP
 are allocated by the caller with ``torch.empty``.  There is NO fallback: if the library cannot be
 loaded, or a tensor is not a contiguous fp32 GPU tensor, the call raises.
 """
+import contextlib
 import ctypes
 import os
 import torch
@@ -11,7 +12,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libspi_hip.so')
 _lib = None
-ABI_VERSION = 13          # SPI_ABI_VERSION of include/spi_hip.h this binding was written against
+ABI_VERSION = 14          # SPI_ABI_VERSION of include/spi_hip.h this binding was written against
 
 c_f = ctypes.c_float
 c_i = ctypes.c_int
@@ -41,6 +42,28 @@ class ModulateJob(ctypes.Structure):
 
 
 MODULATE_MAX_JOBS = 32
+
+
+class NormResidualDesc(ctypes.Structure):
+    """spi_norm_residual_desc of include/spi_hip.h"""
+    _fields_ = [('rows', c_l), ('rows_per_sample', c_l), ('width', c_i), ('dtype', c_i), ('weight_dtype', c_i), ('gate_dtype', c_i), ('gate_mode', c_i),
+                ('gate_act', c_i), ('layer', c_i), ('after', c_i), ('before', c_i), ('scale', c_f), ('eps', c_f), ('h', c_p), ('residual', c_p), ('gate', c_p),
+                ('post_weight', c_p), ('post_bias', c_p), ('pre_weight', c_p), ('pre_bias', c_p), ('stream_out', c_p), ('normed', c_p), ('q', c_p), ('q_scale', c_p),
+                ('q_stride', c_l), ('stats', c_p), ('d_stream', c_p), ('d_normed', c_p), ('d_h', c_p), ('d_residual', c_p), ('d_gate', c_p), ('d_post_weight', c_p),
+                ('d_post_bias', c_p), ('d_pre_weight', c_p), ('d_pre_bias', c_p), ('workspace', c_p), ('workspace_bytes', c_l)]
+
+
+class LinearInt8Desc(ctypes.Structure):
+    """spi_linear_int8_desc of include/spi_hip.h"""
+    _fields_ = [('M', c_l), ('N', c_i), ('K', c_i), ('x_dtype', c_i), ('y_dtype', c_i), ('x_stride', c_l), ('w_stride', c_l), ('w_bytes', c_l), ('x', c_p),
+                ('x_scale', c_p), ('w', c_p), ('w_scale', c_p), ('bias', c_p), ('y', c_p), ('act', c_i), ('alpha', c_f), ('gain', c_f), ('clamp', c_f), ('workspace', c_p),
+                ('workspace_bytes', c_l)]
+
+
+class GroupedLinearDesc(ctypes.Structure):
+    """spi_grouped_linear_desc of include/spi_hip.h"""
+    _fields_ = [('T', c_l), ('E', c_i), ('N', c_i), ('K', c_i), ('dtype', c_i), ('gain', c_f), ('x', c_p), ('w', c_p), ('bias', c_p), ('offsets', c_p), ('y', c_p),
+                ('dy', c_p), ('dx', c_p), ('dw', c_p), ('db', c_p), ('workspace', c_p), ('workspace_bytes', c_l)]
 
 _SIGS = {
     'spi_abi_version': ([], c_i),
@@ -107,6 +130,19 @@ _SIGS = {
     'spi_modulate_multi_bwd': ([ctypes.POINTER(ModulateJob), c_i, c_i, c_p], c_i),
     'spi_affine_multi_fwd': ([ctypes.POINTER(AffineJob), c_i, c_i, c_i, c_l, c_p], c_i),
     'spi_affine_multi_bwd': ([ctypes.POINTER(AffineJob), c_i, c_i, c_i, c_l, c_p], c_i),
+    'spi_sizeof_norm_residual_desc': ([], c_i),
+    'spi_norm_residual_fwd': ([ctypes.POINTER(NormResidualDesc), c_p], c_i),
+    'spi_norm_residual_bwd_workspace': ([ctypes.POINTER(NormResidualDesc)], c_l),
+    'spi_norm_residual_bwd': ([ctypes.POINTER(NormResidualDesc), c_p], c_i),
+    'spi_quantize_rows': ([c_p, c_l, c_i, c_l, c_i, c_p, c_l, c_p, c_p], c_i),
+    'spi_sizeof_linear_int8_desc': ([], c_i),
+    'spi_linear_int8_workspace': ([ctypes.POINTER(LinearInt8Desc)], c_l),
+    'spi_linear_int8': ([ctypes.POINTER(LinearInt8Desc), c_p], c_i),
+    'spi_sizeof_grouped_linear_desc': ([], c_i),
+    'spi_grouped_linear_workspace': ([ctypes.POINTER(GroupedLinearDesc), c_i], c_l),
+    'spi_grouped_linear_fwd': ([ctypes.POINTER(GroupedLinearDesc), c_p], c_i),
+    'spi_grouped_linear_dgrad': ([ctypes.POINTER(GroupedLinearDesc), c_p], c_i),
+    'spi_grouped_linear_wgrad': ([ctypes.POINTER(GroupedLinearDesc), c_p], c_i),
     'spi_adam_multi_dev': ([c_p, c_p, c_i, c_l, c_p, c_f, c_f, c_f, c_p], c_i),
 }
 EXPORTS = sorted(list(_SIGS) + ['spi_last_error'])
@@ -128,12 +164,41 @@ def lib():
         if L.spi_abi_version() != ABI_VERSION or L.spi_sizeof_conv_desc() != ctypes.sizeof(ConvDesc):
             raise RuntimeError('libspi_hip.so ABI mismatch (version %d, spi_conv_desc %d bytes; this binding: version %d, %d bytes): rebuild with '
                                '`python -m spi_amd.csrc.build`' % (L.spi_abi_version(), L.spi_sizeof_conv_desc(), ABI_VERSION, ctypes.sizeof(ConvDesc)))
+        for size, desc in ((L.spi_sizeof_norm_residual_desc, NormResidualDesc), (L.spi_sizeof_linear_int8_desc, LinearInt8Desc),
+                           (L.spi_sizeof_grouped_linear_desc, GroupedLinearDesc)):
+            if size() != ctypes.sizeof(desc):
+                raise RuntimeError(f'libspi_hip.so ABI mismatch ({desc.__name__}: {size()} bytes, this binding: {ctypes.sizeof(desc)}): rebuild with '
+                                   '`python -m spi_amd.csrc.build`')
         _lib = L
     return _lib
 
 
 _PTR_DTYPES = (torch.float32, torch.int32, torch.int64, torch.uint8, torch.float16, torch.float64)      # (float16: the typed entry points / spi_conv_desc.act_dtype only)
 DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.float64: 2}          # SPI_DTYPE_* of the typed plugin entry points (spi_bias_act_t, spi_upfirdn2d_t)
+
+
+ROW_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 3}        # ... of the row operators (spi_norm_residual_*, spi_linear_int8, spi_grouped_linear_*)
+DTYPE_I8 = 4
+
+
+def same_device(*tensors):
+    """The GPU that all given tensors (None: absent) live on; raises if there is a CPU tensor or a second device among them."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError('spi_amd kernels need GPU tensors (no CPU fallback); got a %s tensor' % t.device.type)
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise RuntimeError(f'tensors on different devices: {device} and {t.device}')
+    return device
+
+
+def on(device):
+    """Context in which `device` is the current one: launches go to ITS current stream, workspaces come from its memory."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr_any(t):

@@ -1,0 +1,101 @@
+"""Fully connected layers in 8-bit integers, with a scale for each row (token) and each output channel.
+
+    y = clamp(act(x_scale * weight_scale * (q @ weight_q.T) + bias) * gain)
+
+For FROZEN layers (stage 1 and the mapping network never change their weights): ``quantize_rows`` lays a weight ``[out, in]`` out once, ``linear_int8`` takes
+the layer's place, with the activations of ``bias_act`` in its epilogue.  The integer sums are exact; the only losses are the two roundings to 8 bits.
+"""
+import ctypes
+import torch
+from ... import hip
+from . import bias_act as _ba
+
+MAX_IN_FEATURES = 131071         # SPI_LINEAR_INT8_MAX_K: 127 * 127 * in_features stays below 2^31
+
+
+def _rows(x, name):
+    """[..., K] -> [rows, K] with a row stride of at least K and adjacent values"""
+    k = x.shape[-1]
+    x = x.reshape(-1, k)
+    return x if (k == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or x.stride(0) >= k) else x.contiguous()
+
+
+def _stride(x):
+    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+
+
+def quantize_rows(x):
+    """x [..., K] (fp32 / fp16 / bf16) -> (q int8 [..., K], scale fp32 [...]): ``scale = max|row| / 127``, ``q = round(row / scale)``, ties to even, the division in
+    fp32.  A row of zeros has scale 0; a row that holds an infinity or NaN has scale NaN (so its products are NaN) and q = 0.  The rows of q begin on 16 bytes:
+    q is a view of a buffer with K rounded up to 16."""
+    if x.ndim < 1 or not 1 <= x.shape[-1] <= MAX_IN_FEATURES:
+        raise ValueError(f'rows of {tuple(x.shape)[-1:]} values: 1 to {MAX_IN_FEATURES}')
+    if x.dtype not in hip.ROW_DTYPES:
+        raise TypeError(f'rows of {x.dtype}: float32, float16 or bfloat16')
+    device = hip.same_device(x)
+    k = x.shape[-1]
+    pitch = (k + 15) // 16 * 16
+    with hip.on(device):
+        q = torch.empty(x.shape[:-1] + (pitch,), device=device, dtype=torch.int8)
+        scale = torch.empty(x.shape[:-1], device=device, dtype=torch.float32)
+        r = _rows(x.detach(), 'x')
+        hip.call('spi_quantize_rows', r.data_ptr(), r.shape[0], k, _stride(r), hip.ROW_DTYPES[x.dtype], q.data_ptr(), pitch, scale.data_ptr(), hip.stream())
+    return (q if pitch == k else q[..., :k]), scale
+
+
+def linear_int8(x, weight_q, weight_scale, bias=None, x_scale=None, act='linear', alpha=None, gain=None, clamp=None, out_dtype=None):
+    """x [..., K] -> y [..., N].
+
+    x             fp32 / fp16 / bf16 rows, quantised by the call as ``quantize_rows`` does, or int8 rows with their ``x_scale`` [...] (fp32)
+    weight_q      int8 [N, K] and weight_scale fp32 [N], from ``quantize_rows(weight)``; rows that do not begin on 16 bytes are copied by every call
+    bias          [N] (fp32) or None;  act, alpha, gain, clamp as in ``bias_act``
+    out_dtype     fp32 / fp16 / bf16; default: x's type, fp32 for int8 rows
+
+    Inference only: the rounding has no gradient, so a call that would have to record one raises."""
+    if act not in _ba.activation_funcs:
+        raise KeyError(act)
+    act_id, d_alpha, d_gain, _ = _ba.activation_funcs[act]
+    if weight_q.ndim != 2 or weight_q.dtype != torch.int8 or 0 in weight_q.shape:
+        raise ValueError(f'weight_q {tuple(weight_q.shape)} {weight_q.dtype}: int8 [out_features, in_features]')
+    n, k = weight_q.shape
+    if x.ndim < 1 or x.shape[-1] != k:
+        raise ValueError(f'rows {tuple(x.shape)} for a weight {tuple(weight_q.shape)}')
+    if k > MAX_IN_FEATURES:
+        raise ValueError(f'{k} in_features: at most {MAX_IN_FEATURES} (the sums are 32-bit integers)')
+    if weight_scale.shape != (n,) or weight_scale.dtype != torch.float32:
+        raise ValueError(f'weight_scale {tuple(weight_scale.shape)} {weight_scale.dtype}: float32 [{n}]')
+    if bias is not None and (bias.shape != (n,) or bias.dtype != torch.float32):
+        raise ValueError(f'bias {tuple(bias.shape)} {bias.dtype}: float32 [{n}]')
+    int_rows = x.dtype == torch.int8
+    if int_rows:
+        if x_scale is None or x_scale.shape != x.shape[:-1] or x_scale.dtype != torch.float32:
+            raise ValueError(f'int8 rows {tuple(x.shape)} want x_scale, float32 {tuple(x.shape[:-1])}')
+    elif x_scale is not None:
+        raise ValueError('x_scale belongs to int8 rows')
+    elif x.dtype not in hip.ROW_DTYPES:
+        raise TypeError(f'rows of {x.dtype}: float32, float16, bfloat16 or int8')
+    out_dtype = out_dtype or (torch.float32 if int_rows else x.dtype)
+    if out_dtype not in hip.ROW_DTYPES:
+        raise TypeError(f'out_dtype {out_dtype}: float32, float16 or bfloat16')
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias, x_scale)):
+        raise RuntimeError('linear_int8: rounded rows have no gradient; call it under torch.no_grad() or on tensors that need none')
+    device = hip.same_device(x, weight_q, weight_scale, bias, x_scale)
+    with hip.on(device):
+        y = torch.empty(x.shape[:-1] + (n,), device=device, dtype=out_dtype)
+        r, w = _rows(x, 'x'), _rows(weight_q, 'weight_q')
+        m = r.shape[0]
+        if m == 0:
+            return y
+        weight_scale = weight_scale.contiguous()
+        bias = None if bias is None else bias.contiguous()
+        x_scale = None if x_scale is None else x_scale.contiguous()
+        d = hip.LinearInt8Desc(m, n, k, hip.DTYPE_I8 if int_rows else hip.ROW_DTYPES[x.dtype], hip.ROW_DTYPES[out_dtype], _stride(r), _stride(w),
+                               w.untyped_storage().nbytes() - w.storage_offset(), r.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w.data_ptr(),
+                               weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), act_id, float(d_alpha if alpha is None else alpha),
+                               float(d_gain if gain is None else gain), float(-1 if clamp is None else clamp))
+        nbytes = hip.lib().spi_linear_int8_workspace(ctypes.byref(d))
+        if nbytes:
+            workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
+            d.workspace, d.workspace_bytes = workspace.data_ptr(), nbytes
+        hip.call('spi_linear_int8', ctypes.byref(d), hip.stream())
+    return y
