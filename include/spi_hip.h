@@ -566,9 +566,10 @@ int spi_norm_residual_bwd(const spi_norm_residual_desc* d, spi_stream_t stream);
  * (width <= q_stride; the bytes up to min(q_stride, width rounded up to 16) are written as 0). */
 int spi_quantize_rows(const void* x, int64_t rows, int width, int64_t x_stride, int dtype, int8_t* q, int64_t q_stride, float* scale, spi_stream_t stream);
 
-/* y [M,N] = clamp(act(x_scale[m] * w_scale[n] * sum_k q[m,k] w[n,k] + bias[n]) * gain), the sum in 32-bit integers (exact: K <= SPI_LINEAR_INT8_MAX_K).
+/* y [M,N] = clamp(act(x_scale[m] * w_scale[n] * sum_k q[m,k] w[n,k] + bias[n]) * gain), the sum in 32-bit integers (exact: K <= SPI_LINEAR_INT8_MAX_K).  8-bit rows are at
+ * most 2^22 bytes apart.
  * x: int8 rows (x_dtype = SPI_DTYPE_I8, x_scale given), or rows of fp32 / fp16 / bf16, which the call quantises as spi_quantize_rows does.
- * x rows x_stride elements, w rows w_stride bytes apart; y contiguous, of type y_dtype; bias fp32 or NULL; act: any SPI_ACT_*.
+ * x rows x_stride elements, w rows w_stride bytes apart (any alignment; fastest where rows begin on 16 bytes); y contiguous, of type y_dtype; bias fp32 or NULL; act: any SPI_ACT_*.
  * w_bytes: bytes that may be read from w (>= (N-1) * w_stride + K).  workspace: spi_linear_int8_workspace(d) bytes. */
 #define SPI_LINEAR_INT8_MAX_K 131071
 typedef struct spi_linear_int8_desc {

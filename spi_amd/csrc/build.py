@@ -10,7 +10,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
 SOURCES = ['elementwise.hip', 'render.hip', 'conv.hip', 'winograd.hip', 'losses.hip', 'flrelu.hip', 'hconv.hip', 'norm.hip', 'linear.hip']
-HEADERS = ['common.hpp', 'typed.hpp']
+HEADERS = ['common.hpp', 'typed.hpp', 'tile.hpp']
 # winograd.hip keeps its 256 accumulators per lane in AGPRs (the other 256 registers hold operands and the loaders' state)
 NO_VGPR_FORM = {'winograd.hip'}
 # Some forms of the packed fp32 instructions that hipcc makes out of ordinary float code have given wrong results on this hardware now and then: these files

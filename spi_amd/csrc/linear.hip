@@ -1,41 +1,9 @@
 // Products of rows with weights: 8-bit integers with scales for each row and each output (spi_linear_int8) and ragged groups of rows with a weight each
-// (spi_grouped_linear_*).  Matrix-core tiles: every operand enters v_mfma_*_32x32x* as 16-byte chunks along the summed axis, whatever its type.
-#include "typed.hpp"
+// (spi_grouped_linear_*).
+#include "tile.hpp"
 #include <algorithm>
 
 namespace {
-
-// ---- 32x32 tile steps: lane l holds 16 bytes of row (l & 31), chunk half (l >> 5); result register r of lane l is row 8 (r >> 2) + 4 (l >> 5) + (r & 3) of A,
-// row (l & 31) of B ------------------------------------------------------------------------------------------------------------------------
-template <typename T> struct Mma;
-template <> struct Mma<half_t> {
-    typedef f32x16_acc Acc;
-    typedef half_t V __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ Acc step(i32x4_t a, i32x4_t b, Acc c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
-    }
-};
-template <> struct Mma<bf16_t> {
-    typedef f32x16_acc Acc;
-    typedef bf16_t V __attribute__((ext_vector_type(8)));
-    static __device__ __forceinline__ Acc step(i32x4_t a, i32x4_t b, Acc c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b), c, 0, 0, 0);
-    }
-};
-template <> struct Mma<float> {                                 // four steps of two: values j of both halves' chunks are summed together
-    typedef f32x16_acc Acc;
-    typedef float V __attribute__((ext_vector_type(4)));
-    static __device__ __forceinline__ Acc step(i32x4_t a, i32x4_t b, Acc c) {
-        const V x = __builtin_bit_cast(V, a), y = __builtin_bit_cast(V, b);          // (whole vectors: a bit cast of one element reads element 0)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
-        return c;
-    }
-};
-template <> struct Mma<int8_t> {
-    typedef i32x16_acc Acc;
-    static __device__ __forceinline__ Acc step(i32x4_t a, i32x4_t b, Acc c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
-};
 
 // ---- groups ------------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ int wave_scan_max(int v) {                         // inclusive running maximum over the lanes of a wave
@@ -46,6 +14,8 @@ __device__ __forceinline__ int wave_scan_max(int v) {                         //
     }
     return v;
 }
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }      // the same in all lanes: into a scalar register
 
 // A tile of rows: group e, or e = -1 for rows of no group.
 struct RowTile { int e, row, end; };
@@ -69,12 +39,27 @@ __device__ RowTile find_tile(const int32_t* __restrict__ offsets, int E, int T, 
             const int l = __builtin_ctzll(hit);
             const int first = __shfl(upto - n, l), s = __shfl(start, l), e = __shfl(end, l);
             const int range = b + l;
-            return RowTile{range == 0 || range == E + 1 ? -1 : range - 1, s + (tile - first) * BM, e};
+            return RowTile{uniform(range == 0 || range == E + 1 ? -1 : range - 1), uniform(s + (tile - first) * BM), uniform(e)};
         }
         carry = __shfl(end, 63);
         before = __shfl(upto, 63);
     }
     return RowTile{-1, 0, 0};
+}
+// number of tiles that find_tile knows
+__device__ int count_tiles(const int32_t* __restrict__ offsets, int E, int T, int BM) {
+    const int lane = threadIdx.x & 63;
+    int carry = 0, tiles = 0;
+    for (int b = 0; b <= E + 1; b += 64) {
+        const int i = b + lane;
+        int end = i <= E ? min(max(offsets[i], 0), T) : T;
+        end = max(wave_scan_max(end), carry);
+        int start = __shfl_up(end, 1);
+        if (lane == 0) start = carry;
+        tiles += __shfl(wave_scan_add(i <= E + 1 ? (end - start + BM - 1) / BM : 0), 63);
+        carry = __shfl(end, 63);
+    }
+    return uniform(tiles);
 }
 // rows of group e, by the same reading of the offsets
 __device__ RowTile group_rows(const int32_t* __restrict__ offsets, int T, int e) {
@@ -82,60 +67,10 @@ __device__ RowTile group_rows(const int32_t* __restrict__ offsets, int T, int e)
     int start = 0;
     for (int i = lane; i <= e; i += 64) start = max(start, min(max(offsets[i], 0), T));
     start = __shfl(wave_scan_max(start), 63);
-    return RowTile{e, start, max(start, min(max(offsets[e + 1], 0), T))};
+    return RowTile{e, uniform(start), uniform(max(start, min(max(offsets[e + 1], 0), T)))};
 }
 // tiles that T rows in E groups can need
 int64_t most_tiles(int64_t T, int E, int BM) { return T / BM + E + 2; }
-
-// ---- one 64 x 64 tile, any strides --------------------------------------------------------------------------------------------------------
-// An operand: value (i, k) at p[i * si + k * sk], i < ni, k < nk; one of the strides is 1.
-template <typename T> struct Operand { const T* p; int64_t si, sk; int ni, nk; };
-constexpr int PITCH = 144;                                                     // bytes of an LDS row: 128 and a chunk that spreads the banks
-
-template <typename T>
-__device__ __forceinline__ void stage_operand(const Operand<T>& o, int k0, char* lds) {
-    constexpr int N = Chunk<T>::N, KT = 128 / (int)sizeof(T);
-    if (o.sk == 1) {
-#pragma unroll
-        for (int it = 0; it < 2; ++it) {
-            const int id = threadIdx.x + it * 256, i = id >> 3, c = id & 7, k = k0 + c * N;
-            const Chunk<T> v = load_chunk(o.p + (i < o.ni ? i : 0) * o.si + k, i < o.ni ? o.nk - k : 0);
-            *reinterpret_cast<i32x4_t*>(lds + i * PITCH + c * 16) = __builtin_bit_cast(i32x4_t, v);
-        }
-    } else {
-#pragma unroll
-        for (int it = 0; it < 2; ++it) {
-            const int id = threadIdx.x + it * 256, k = id % KT, i = (id / KT) * N;      // KT * 64 / N = 512 chunks
-            const Chunk<T> v = load_chunk(o.p + (int64_t)(k0 + k < o.nk ? k0 + k : 0) * o.sk + i, k0 + k < o.nk ? o.ni - i : 0);
-#pragma unroll
-            for (int j = 0; j < N; ++j) *reinterpret_cast<T*>(lds + (i + j) * PITCH + k * (int)sizeof(T)) = v.v[j];
-        }
-    }
-}
-
-template <typename T>
-__device__ __forceinline__ void tile64(const Operand<T>& A, const Operand<T>& B, char* lds, typename Mma<T>::Acc& acc) {
-    constexpr int KT = 128 / (int)sizeof(T);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-    const char* pa = lds + (wm * 32 + (lane & 31)) * PITCH + (lane >> 5) * 16;
-    const char* pb = lds + 64 * PITCH + (wn * 32 + (lane & 31)) * PITCH + (lane >> 5) * 16;
-    for (int k0 = 0; k0 < A.nk; k0 += KT) {
-        __syncthreads();
-        stage_operand(A, k0, lds);
-        stage_operand(B, k0, lds + 64 * PITCH);
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-            acc = Mma<T>::step(*reinterpret_cast<const i32x4_t*>(pa + c * 32), *reinterpret_cast<const i32x4_t*>(pb + c * 32), acc);
-    }
-}
-// f(i, j, value) for the values of this thread's part of the tile
-template <typename Acc, typename F>
-__device__ __forceinline__ void tile64_out(const Acc& acc, F f) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) f(wm * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3), wn * 32 + (lane & 31), acc[r]);
-}
 
 // ---- 8-bit integers ----------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float linear_act(int act, float alpha, float x) {
@@ -165,14 +100,29 @@ __device__ __forceinline__ float int8_epilogue(const Int8Args& a, int acc, float
     return v;
 }
 
-__global__ void __launch_bounds__(256) int8_tile64_kernel(const Int8Args a) {
-    __shared__ __attribute__((aligned(16))) char lds[2 * 64 * PITCH];
-    const int m0 = blockIdx.x * 64, n0 = blockIdx.y * 64;
-    i32x16_acc acc = {};
-    tile64<int8_t>({a.q + (int64_t)m0 * a.q_stride, a.q_stride, 1, a.M - m0, a.K}, {a.w + (int64_t)n0 * a.w_stride, a.w_stride, 1, a.N - n0, a.K}, lds, acc);
-    tile64_out(acc, [&](int i, int j, int v) {
-        const int m = m0 + i, n = n0 + j;
-        if (m < a.M && n < a.N) store_f32(a.y, a.y_dtype, (int64_t)m * a.N + n, int8_epilogue(a, v, a.q_scale[m], a.w_scale[n], a.bias ? a.bias[n] : 0.f));
+// Tiles of 256 x 256 (8 waves), 128 x 128 and 64 x 64 (4 waves).
+template <typename T, int SIZE, bool COLA, bool COLB, bool DMA>
+using Engine = TileEngine<T, SIZE, SIZE, 2, SIZE == 256 ? 4 : 2, COLA, COLB, DMA>;
+
+template <int SIZE, bool DMA>
+__global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) int8_tile_kernel(const Int8Args a, int rows, int cols) {
+    typedef Engine<int8_t, SIZE, false, false, DMA> E;
+    __shared__ __attribute__((aligned(1024))) char s0[E::STAGE], s1[E::STAGE];
+    int row, col;
+    band_order(xcd_run(blockIdx.x, gridDim.x), rows, cols, row, col);
+    const int m0 = row * SIZE, n0 = col * SIZE, m = min(SIZE, a.M - m0), n = min(SIZE, a.N - n0);
+    typename E::Accs acc = {};
+    const int64_t k = DMA ? (a.K + 15) / 16 * 16 : a.K;                        // (DMA: the padding of the quantised rows is 0, so that of the weights does not count)
+    const TileOperand A{(const char*)a.q + m0 * a.q_stride, a.q_stride, m * a.q_stride, k, m}, B{(const char*)a.w + n0 * a.w_stride, a.w_stride, n * a.w_stride, k, n};
+    E::run(A, B, s0, s1, acc);
+    E::each(acc, s0, s1, [&](int i, int j, i32x4_t v) {
+        if (i >= m || j >= n) return;
+        const float scale = a.q_scale[m0 + i];
+        const int c0 = n0 + j;
+        float y[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = j + c < n ? int8_epilogue(a, v[c], scale, a.w_scale[c0 + c], a.bias ? a.bias[c0 + c] : 0.f) : 0.f;
+        store_f32x4(a.y, a.y_dtype, (int64_t)(m0 + i) * a.N + c0, y, n - j);
     });
 }
 
@@ -250,7 +200,7 @@ void quantize_any(const void* x, int64_t rows, int width, int64_t x_stride, int 
 
 int check_int8(const spi_linear_int8_desc* d, const char* who) {
     SPI_REQUIRE(d, "%s: no descriptor", who);
-    SPI_REQUIRE(d->M >= 0 && d->M < (1ll << 31) - 64 && d->N >= 1 && d->N <= 65535 * 64 && d->K >= 1 && d->K <= SPI_LINEAR_INT8_MAX_K, "%s: M %lld, N %d, K %d", who,
+    SPI_REQUIRE(d->M >= 0 && d->M < (1ll << 31) - 64 && d->N >= 1 && d->K >= 1 && d->K <= SPI_LINEAR_INT8_MAX_K && ceil_div64(d->M, 64) * ceil_div64(d->N, 64) < (1ll << 31), "%s: M %lld, N %d, K %d", who,
                 (long long)d->M, d->N, d->K);
     SPI_REQUIRE(d->x_dtype == SPI_DTYPE_I8 || float_rows(d->x_dtype), "%s: x_dtype %d", who, d->x_dtype);
     SPI_REQUIRE(float_rows(d->y_dtype), "%s: y_dtype %d", who, d->y_dtype);
@@ -258,6 +208,8 @@ int check_int8(const spi_linear_int8_desc* d, const char* who) {
     SPI_REQUIRE(d->w && d->w_scale && (d->x_dtype != SPI_DTYPE_I8 || d->x_scale || d->M == 0), "%s: null weights or scales", who);
     SPI_REQUIRE(d->x_stride >= d->K && d->w_stride >= d->K && d->w_bytes >= (int64_t)(d->N - 1) * d->w_stride + d->K, "%s: strides %lld, %lld", who, (long long)d->x_stride,
                 (long long)d->w_stride);
+    SPI_REQUIRE(d->w_stride <= (1 << 22) && (d->x_dtype != SPI_DTYPE_I8 || d->x_stride <= (1 << 22)), "%s: 8-bit rows %lld, %lld bytes apart (at most 2^22)", who,
+                (long long)d->x_stride, (long long)d->w_stride);
     SPI_REQUIRE(d->act >= SPI_ACT_LINEAR && d->act <= SPI_ACT_SWISH, "%s: act %d", who, d->act);
     return SPI_OK;
 }
@@ -272,65 +224,176 @@ struct GroupArgs {
     float gain;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) grouped_fwd64_kernel(const GroupArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[2 * 64 * PITCH];
-    const RowTile t = find_tile(a.offsets, a.E, a.T, 64, blockIdx.x);
-    if (t.row >= t.end) return;
-    const int n0 = blockIdx.y * 64;
-    f32x16_acc acc = {};
-    if (t.e >= 0)
-        tile64<T>({(const T*)a.x + (int64_t)t.row * a.K, a.K, 1, t.end - t.row, a.K}, {(const T*)a.w + ((int64_t)t.e * a.N + n0) * a.K, a.K, 1, a.N - n0, a.K}, lds, acc);
-    tile64_out(acc, [&](int i, int j, float v) {
-        const int row = t.row + i, n = n0 + j;
-        if (row < t.end && n < a.N)
-            ((T*)a.y)[(int64_t)row * a.N + n] = (T)(t.e < 0 ? 0.f : v * a.gain + (a.bias ? (float)((const T*)a.bias)[(int64_t)t.e * a.N + n] : 0.f));
-    });
-}
-template <typename T>
-__global__ void __launch_bounds__(256) grouped_dgrad64_kernel(const GroupArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[2 * 64 * PITCH];
-    const RowTile t = find_tile(a.offsets, a.E, a.T, 64, blockIdx.x);
-    if (t.row >= t.end) return;
-    const int k0 = blockIdx.y * 64;
-    f32x16_acc acc = {};
-    if (t.e >= 0)
-        tile64<T>({(const T*)a.dy + (int64_t)t.row * a.N, a.N, 1, t.end - t.row, a.N}, {(const T*)a.w + (int64_t)t.e * a.N * a.K + k0, 1, a.K, a.K - k0, a.N}, lds, acc);
-    tile64_out(acc, [&](int i, int j, float v) {
-        const int row = t.row + i, k = k0 + j;
-        if (row < t.end && k < a.K) ((T*)a.dx)[(int64_t)row * a.K + k] = (T)(v * a.gain);
-    });
-}
-template <typename T>
-__global__ void __launch_bounds__(256) grouped_wgrad64_kernel(const GroupArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[2 * 64 * PITCH];
-    const int n0 = blockIdx.x * 64, k0 = blockIdx.y * 64, e = blockIdx.z;
-    const RowTile t = group_rows(a.offsets, a.T, e);
-    f32x16_acc acc = {};
-    tile64<T>({(const T*)a.dy + (int64_t)t.row * a.N + n0, 1, a.N, a.N - n0, t.end - t.row}, {(const T*)a.x + (int64_t)t.row * a.K + k0, 1, a.K, a.K - k0, t.end - t.row}, lds, acc);
-    tile64_out(acc, [&](int i, int j, float v) {
-        const int n = n0 + i, k = k0 + j;
-        if (n < a.N && k < a.K) ((T*)a.dw)[((int64_t)e * a.N + n) * a.K + k] = (T)(v * a.gain);
-    });
-}
-// db[e][n] = sum of dy over the group's rows: 64 columns per block, four rows at a time, in a fixed order
-template <typename T>
-__global__ void __launch_bounds__(256) grouped_bias_grad_kernel(const GroupArgs a) {
-    __shared__ float s[4][64];
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c, e = blockIdx.y;
-    const RowTile t = group_rows(a.offsets, a.T, e);
-    float v = 0.f;
-    if (n < a.N)
-        for (int row = t.row + r; row < t.end; row += 4) v += (float)((const T*)a.dy)[(int64_t)row * a.N + n];
-    s[r][c] = v;
-    __syncthreads();
-    if (r == 0 && n < a.N) ((T*)a.db)[(int64_t)e * a.N + n] = (T)((s[0][c] + s[1][c]) + (s[2][c] + s[3][c]));
+enum { PASS_FWD = 0, PASS_DGRAD = 1, PASS_WGRAD = 2 };
+template <typename T, int PASS, int SIZE, bool DMA>
+using PassEngine = Engine<T, SIZE, PASS == PASS_WGRAD, PASS != PASS_FWD, DMA>;
+
+// the tile of engine E at rows t.row .. (at most t.end), columns c0 ..; of dw: at (r0, c0) of group t.e
+template <typename E, typename T, int PASS>
+__device__ __forceinline__ void grouped_tile(const GroupArgs& a, const RowTile& t, int r0, int c0, char* s0, char* s1) {
+    constexpr int ES = (int)sizeof(T);
+    const int64_t pn = (int64_t)a.N * ES, pk = (int64_t)a.K * ES;
+    const int width = PASS == PASS_FWD ? a.N : a.K, cols = min(E::BN, width - c0);
+    typename E::Accs acc = {};
+    auto run = [&](const TileOperand& A, const TileOperand& B) { E::run(A, B, s0, s1, acc); };
+    if constexpr (PASS == PASS_WGRAD) {
+        const int rows = min(E::BM, a.N - r0);
+        const int64_t len = t.end - t.row;
+        run({(const char*)a.dy + t.row * pn + r0 * ES, pn, len * pn - r0 * ES, len, rows}, {(const char*)a.x + t.row * pk + c0 * ES, pk, len * pk - c0 * ES, len, cols});
+        E::each(acc, s0, s1, [&](int i, int j, f32x4_t v) {
+            if (i >= rows || j >= cols) return;
+            const float y[4] = {v[0] * a.gain, v[1] * a.gain, v[2] * a.gain, v[3] * a.gain};
+            store_row4((T*)a.dw + ((int64_t)t.e * a.N + r0 + i) * a.K + c0 + j, y, cols - j);
+        });
+    } else {
+        const int rows = min(E::BM, t.end - t.row), inner = PASS == PASS_FWD ? a.K : a.N;
+        if (t.e >= 0) {
+            const int64_t pi = PASS == PASS_FWD ? pk : pn;
+            const char* w = (const char*)a.w + (int64_t)t.e * a.N * pk;
+            const TileOperand A{(const char*)(PASS == PASS_FWD ? a.x : a.dy) + t.row * pi, pi, rows * pi, inner, rows};
+            if constexpr (PASS == PASS_FWD) run(A, {w + c0 * pk, pk, cols * pk, inner, cols});
+            else run(A, {w + c0 * ES, pk, inner * pk - c0 * ES, inner, cols});
+        }
+        const T* bias = PASS == PASS_FWD && a.bias && t.e >= 0 ? (const T*)a.bias + (int64_t)t.e * a.N + c0 : nullptr;
+        T* out = (T*)(PASS == PASS_FWD ? a.y : a.dx) + (int64_t)t.row * width + c0;
+        E::each(acc, s0, s1, [&](int i, int j, f32x4_t v) {
+            if (i >= rows || j >= cols) return;
+            float y[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) y[q] = v[q] * a.gain + (bias && j + q < cols ? (float)bias[j + q] : 0.f);
+            store_row4(out + (int64_t)i * width + j, y, cols - j);
+        });
+    }
 }
 
+// One tile a block.  Tiles of 256 x 256 come in rounds of one for each CU; where the last round would leave more than half of the chip idle, its tiles are cut into four.
+constexpr int CUS = 256;
+__device__ __forceinline__ int whole_tiles(int tiles) { const int last = tiles % CUS; return last <= CUS / 2 ? tiles - last : tiles; }
+int64_t most_blocks(int64_t tiles) { return tiles + 3 * (CUS / 2); }
+
+template <typename T, int PASS, int SIZE, bool DMA>
+__global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) grouped_tile_kernel(const GroupArgs a) {
+    typedef PassEngine<T, PASS, SIZE, DMA> E;
+    __shared__ __attribute__((aligned(1024))) char s0[E::STAGE], s1[E::STAGE];
+    const int width = PASS == PASS_FWD ? a.N : a.K, cols = (width + SIZE - 1) / SIZE;
+    const int rows = PASS == PASS_WGRAD ? (a.N + SIZE - 1) / SIZE : count_tiles(a.offsets, a.E, a.T, SIZE), tiles = rows * cols * (PASS == PASS_WGRAD ? a.E : 1);
+    const int whole = SIZE == 256 ? whole_tiles(tiles) : tiles, cut = (int)blockIdx.x - whole;
+    const int tile = cut < 0 ? (int)blockIdx.x : whole + cut / 4;
+    if (tile >= tiles) return;
+    int row, col, r0 = 0;
+    RowTile t;
+    if constexpr (PASS == PASS_WGRAD) {
+        const int of = rows * cols;                            // each group's tiles over all XCDs: groups differ in length
+        band_order(xcd_run(tile % of, of), rows, cols, row, col);
+        t = group_rows(a.offsets, a.T, tile / of);
+        r0 = row * SIZE;
+    } else {
+        band_order(cut < 0 ? xcd_run(tile, whole) : tile, rows, cols, row, col);
+        t = find_tile(a.offsets, a.E, a.T, SIZE, row);
+    }
+    int c0 = col * SIZE;
+    if constexpr (SIZE == 256) {
+        if (cut >= 0) {
+            typedef TileEngine<T, 128, 128, 2, 4, PASS == PASS_WGRAD, PASS != PASS_FWD, DMA> Q;
+            const int down = cut % 4 / 2 * 128, right = cut % 2 * 128;
+            c0 += right;
+            if (PASS == PASS_WGRAD) r0 += down;
+            else t.row += down;
+            if (c0 < width && (PASS == PASS_WGRAD ? r0 < a.N : t.row < t.end)) grouped_tile<Q, T, PASS>(a, t, r0, c0, s0, s1);
+            return;
+        }
+    }
+    grouped_tile<E, T, PASS>(a, t, r0, c0, s0, s1);
+}
+// db[e][n] = sum of dy over the group's rows, in two steps of a fixed order: part s of S of the group's rows into part [E][S][N] (S = 1: straight into db), then the
+// parts.  A block takes 64 chunks of 16 bytes by four rows at a time.
+template <typename T>
+__global__ void __launch_bounds__(256) grouped_bias_grad_kernel(const GroupArgs a, float* __restrict__ part, int S) {
+    constexpr int N = Chunk<T>::N;
+    __shared__ float sum[4][64][N + 1];
+    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = (blockIdx.x * 64 + c) * N, s = blockIdx.y, e = blockIdx.z;
+    const RowTile t = group_rows(a.offsets, a.T, e);
+    const int64_t len = t.end - t.row, from = t.row + len * s / S, to = t.row + len * (s + 1) / S;
+    float v[N] = {};
+    if (n < a.N)
+#pragma unroll 4
+        for (int64_t row = from + r; row < to; row += 4) {
+            const Chunk<T> x = load_chunk((const T*)a.dy + row * a.N + n, a.N - n);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] += (float)x.v[j];
+        }
+#pragma unroll
+    for (int j = 0; j < N; ++j) sum[r][c][j] = v[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * N; i += 256) {
+        const int cc = i / N, j = i % N, col = blockIdx.x * 64 * N + i;
+        if (col >= a.N) break;
+        const float x = (sum[0][cc][j] + sum[1][cc][j]) + (sum[2][cc][j] + sum[3][cc][j]);
+        if (S > 1) part[((int64_t)e * S + s) * a.N + col] = x;
+        else ((T*)a.db)[(int64_t)e * a.N + col] = (T)x;
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) grouped_bias_join_kernel(const GroupArgs a, const float* __restrict__ part, int S) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)a.E * a.N) return;
+    const float* p = part + i / a.N * S * a.N + i % a.N;
+    float v = 0.f;
+    for (int s = 0; s < S; ++s) v += p[(int64_t)s * a.N];
+    ((T*)a.db)[i] = (T)v;
+}
+// parts of a group's rows: enough blocks for the chip (four for each CU), no part under 64 rows of an average group
+int bias_parts(const spi_grouped_linear_desc& d) {
+    const int64_t blocks = ceil_div64(d.N, 64 * (d.dtype == SPI_DTYPE_F32 ? 4 : 8)) * d.E;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div64(1024, blocks), d.T / d.E / 64, 64}));
+}
+template <typename T>
+void bias_grad(const spi_grouped_linear_desc& d, const GroupArgs& a, hipStream_t st) {
+    const int S = bias_parts(d);
+    hipLaunchKernelGGL(grouped_bias_grad_kernel<T>, dim3((unsigned)ceil_div64(d.N, 64 * Chunk<T>::N), (unsigned)S, (unsigned)d.E), dim3(256), 0, st, a, (float*)d.workspace, S);
+    if (S > 1) hipLaunchKernelGGL(grouped_bias_join_kernel<T>, dim3((unsigned)ceil_div64((int64_t)d.E * d.N, 256)), dim3(256), 0, st, a, (const float*)d.workspace, S);
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+// Edge of the tiles, from the number of tiles that there would be (`rows`(edge) tile rows).  A tile of 256 reads a fourth of what sixteen of 64 do, but a chip half idle costs
+// more.  Measured, bf16 forward, edges 64 / 128 / 256: 2048 x 1024 x 1024 in 4 groups (144 tiles of 128) 11.4 / 15.8 / 15.5 us, 8192 x 1024 x 1024 in 8 (544, 128 of 256)
+// 32.5 / 25.2 / 31.6, 16384 x 2048 x 2048 in 8 (512 of 256) 307 / 206 / 196; int8 4096^3 (256 of 256) 130 / 105 / 94.  Through registers (rows on odd places) 128 pays later:
+// bf16 weight gradient of 8192 x 1003 x 501 (256 tiles of 128) 37 / 55.
+template <typename F>
+int tile_edge(F rows, int64_t width, bool dma) {
+    if (dma && rows(256) * ceil_div64(width, 256) >= CUS) return 256;
+    return rows(128) * ceil_div64(width, 128) >= (dma ? CUS : CUS * 3 / 2) ? 128 : 64;
+}
+template <typename T, int PASS, int SIZE, bool DMA>
+void launch_tiles(const GroupArgs& a, hipStream_t st) {
+    const int64_t tiles = PASS == PASS_WGRAD ? ceil_div64(a.N, SIZE) * ceil_div64(a.K, SIZE) * a.E : most_tiles(a.T, a.E, SIZE) * ceil_div64(PASS == PASS_FWD ? a.N : a.K, SIZE);
+    hipLaunchKernelGGL((grouped_tile_kernel<T, PASS, SIZE, DMA>), dim3((unsigned)(SIZE == 256 ? most_blocks(tiles) : tiles)), dim3(SIZE == 256 ? 512 : 256), 0, st, a);
+}
+template <typename T, int PASS>
+void grouped_pass(const GroupArgs& a, hipStream_t st) {
+    constexpr int ES = (int)sizeof(T);
+    const bool dma = a.N * ES % 16 == 0 && a.K * ES % 16 == 0 && aligned16(a.x) && aligned16(a.w) && aligned16(a.dy);
+    const int64_t width = PASS == PASS_FWD ? a.N : a.K;
+    auto rows = [&](int size) { return PASS == PASS_WGRAD ? ceil_div64(a.N, size) * a.E : a.T / size + std::min(a.T, a.E) / 2; };        // (of ragged groups half a tile each is empty)
+    const int size = tile_edge(rows, width, dma);
+    if (size == 256) launch_tiles<T, PASS, 256, true>(a, st);
+    else if (size == 128 && dma) launch_tiles<T, PASS, 128, true>(a, st);
+    else if (size == 128) launch_tiles<T, PASS, 128, false>(a, st);
+    else if (dma) launch_tiles<T, PASS, 64, true>(a, st);
+    else launch_tiles<T, PASS, 64, false>(a, st);
+}
+template <int PASS>
+void grouped_pass(int dtype, const GroupArgs& a, hipStream_t st) {
+    if (dtype == SPI_DTYPE_F32) grouped_pass<float, PASS>(a, st);
+    else if (dtype == SPI_DTYPE_F16) grouped_pass<half_t, PASS>(a, st);
+    else grouped_pass<bf16_t, PASS>(a, st);
+}
 int check_grouped(const spi_grouped_linear_desc* d, const char* who) {
     SPI_REQUIRE(d, "%s: no descriptor", who);
-    SPI_REQUIRE(d->T >= 0 && d->T < (1ll << 31) - 64 && d->E >= 1 && d->E <= 65535 && d->N >= 1 && d->N <= 65535 * 64 && d->K >= 1 && d->K <= 65535 * 64,
+    SPI_REQUIRE(d->T >= 0 && d->T < (1ll << 31) - 64 && d->E >= 1 && d->E <= 65535 && d->N >= 1 && d->N <= (1 << 20) && d->K >= 1 && d->K <= (1 << 20),
                 "%s: T %lld, E %d, N %d, K %d", who, (long long)d->T, d->E, d->N, d->K);
+    SPI_REQUIRE((most_tiles(d->T, d->E, 64) * (int64_t)ceil_div64(std::max(d->N, d->K), 64) < (1ll << 31) - 1024) && ceil_div64(d->N, 64) * ceil_div64(d->K, 64) * d->E < (1ll << 31) - 1024,
+                "%s: T %lld, E %d, N %d, K %d are more tiles than a launch has blocks", who, (long long)d->T, d->E, d->N, d->K);
     SPI_REQUIRE(float_rows(d->dtype), "%s: dtype %d", who, d->dtype);
     SPI_REQUIRE(d->offsets, "%s: null offsets", who);
     return SPI_OK;
@@ -370,29 +433,32 @@ extern "C" int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t strea
         quantize_any(d->x, d->M, d->K, d->x_stride, d->x_dtype, (int8_t*)a.q, a.q_stride, (float*)a.q_scale, st);
         SPI_LAUNCH_CHECK("spi_linear_int8 (quantize)");
     }
-    hipLaunchKernelGGL(int8_tile64_kernel, dim3((unsigned)ceil_div64(d->M, 64), (unsigned)ceil_div64(d->N, 64)), dim3(256), 0, st, a);
+    // 16-byte rows; where they do not end on 16 bytes, the rows' own padding has to be 0 and the weights' readable
+    const bool dma = aligned16(a.q) && aligned16(a.w) && a.q_stride % 16 == 0 && a.w_stride % 16 == 0 &&
+                     (d->K % 16 == 0 || (d->x_dtype != SPI_DTYPE_I8 && d->w_bytes >= (int64_t)(d->N - 1) * d->w_stride + q_pitch(d->K)));
+    const int size = tile_edge([&](int edge) { return ceil_div64(d->M, edge); }, d->N, dma), rows = (int)ceil_div64(d->M, size), cols = (int)ceil_div64(d->N, size);
+    const dim3 grid((unsigned)rows * (unsigned)cols);
+    if (size == 256) hipLaunchKernelGGL((int8_tile_kernel<256, true>), grid, dim3(512), 0, st, a, rows, cols);
+    else if (size == 128 && dma) hipLaunchKernelGGL((int8_tile_kernel<128, true>), grid, dim3(256), 0, st, a, rows, cols);
+    else if (size == 128) hipLaunchKernelGGL((int8_tile_kernel<128, false>), grid, dim3(256), 0, st, a, rows, cols);
+    else if (dma) hipLaunchKernelGGL((int8_tile_kernel<64, true>), grid, dim3(256), 0, st, a, rows, cols);
+    else hipLaunchKernelGGL((int8_tile_kernel<64, false>), grid, dim3(256), 0, st, a, rows, cols);
     SPI_LAUNCH_CHECK("spi_linear_int8");
     return SPI_OK;
 }
 
 extern "C" int spi_sizeof_grouped_linear_desc(void) { return (int)sizeof(spi_grouped_linear_desc); }
 extern "C" int64_t spi_grouped_linear_workspace(const spi_grouped_linear_desc* d, int pass) {
-    (void)pass;
-    return check_grouped(d, "spi_grouped_linear_workspace") ? 0 : 0;
+    if (check_grouped(d, "spi_grouped_linear_workspace") || pass != PASS_WGRAD || !d->db) return 0;
+    const int S = bias_parts(*d);
+    return S > 1 ? (int64_t)d->E * S * d->N * (int64_t)sizeof(float) : 0;
 }
-#define SPI_BY_TYPE(kernel, grid, args)                                                                                   \
-    do {                                                                                                                  \
-        if (d->dtype == SPI_DTYPE_F32) hipLaunchKernelGGL(kernel<float>, grid, dim3(256), 0, as_stream(stream), args);        \
-        else if (d->dtype == SPI_DTYPE_F16) hipLaunchKernelGGL(kernel<half_t>, grid, dim3(256), 0, as_stream(stream), args);  \
-        else hipLaunchKernelGGL(kernel<bf16_t>, grid, dim3(256), 0, as_stream(stream), args);                                 \
-    } while (0)
-
 extern "C" int spi_grouped_linear_fwd(const spi_grouped_linear_desc* d, spi_stream_t stream) {
     if (int rc = check_grouped(d, "spi_grouped_linear_fwd")) return rc;
     if (d->T == 0) return SPI_OK;
     SPI_REQUIRE(d->x && d->w && d->y, "spi_grouped_linear_fwd: null pointer");
     const GroupArgs a = group_args(*d);
-    SPI_BY_TYPE(grouped_fwd64_kernel, dim3((unsigned)most_tiles(d->T, d->E, 64), (unsigned)ceil_div64(d->N, 64)), a);
+    grouped_pass<PASS_FWD>(d->dtype, a, as_stream(stream));
     SPI_LAUNCH_CHECK("spi_grouped_linear_fwd");
     return SPI_OK;
 }
@@ -401,7 +467,7 @@ extern "C" int spi_grouped_linear_dgrad(const spi_grouped_linear_desc* d, spi_st
     if (d->T == 0) return SPI_OK;
     SPI_REQUIRE(d->dy && d->w && d->dx, "spi_grouped_linear_dgrad: null pointer");
     const GroupArgs a = group_args(*d);
-    SPI_BY_TYPE(grouped_dgrad64_kernel, dim3((unsigned)most_tiles(d->T, d->E, 64), (unsigned)ceil_div64(d->K, 64)), a);
+    grouped_pass<PASS_DGRAD>(d->dtype, a, as_stream(stream));
     SPI_LAUNCH_CHECK("spi_grouped_linear_dgrad");
     return SPI_OK;
 }
@@ -411,11 +477,14 @@ extern "C" int spi_grouped_linear_wgrad(const spi_grouped_linear_desc* d, spi_st
     SPI_REQUIRE(d->T == 0 || !d->dw || d->x, "spi_grouped_linear_wgrad: null x");
     const GroupArgs a = group_args(*d);
     if (d->dw) {
-        SPI_BY_TYPE(grouped_wgrad64_kernel, dim3((unsigned)ceil_div64(d->N, 64), (unsigned)ceil_div64(d->K, 64), (unsigned)d->E), a);
+        grouped_pass<PASS_WGRAD>(d->dtype, a, as_stream(stream));
         SPI_LAUNCH_CHECK("spi_grouped_linear_wgrad");
     }
     if (d->db) {
-        SPI_BY_TYPE(grouped_bias_grad_kernel, dim3((unsigned)ceil_div64(d->N, 64), (unsigned)d->E), a);
+        SPI_REQUIRE(d->workspace_bytes >= spi_grouped_linear_workspace(d, PASS_WGRAD) && (d->workspace || d->workspace_bytes == 0), "spi_grouped_linear_wgrad: workspace too small");
+        if (d->dtype == SPI_DTYPE_F32) bias_grad<float>(*d, a, as_stream(stream));
+        else if (d->dtype == SPI_DTYPE_F16) bias_grad<half_t>(*d, a, as_stream(stream));
+        else bias_grad<bf16_t>(*d, a, as_stream(stream));
         SPI_LAUNCH_CHECK("spi_grouped_linear_wgrad (bias)");
     }
     return SPI_OK;

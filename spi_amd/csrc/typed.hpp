@@ -57,6 +57,21 @@ __device__ __forceinline__ void store_f32(void* base, int dtype, int64_t at, flo
     else if (dtype == SPI_DTYPE_F16) ((half_t*)base)[at] = (half_t)v;
     else ((bf16_t*)base)[at] = (bf16_t)v;
 }
+// four neighbours of a row (the first n of them), rounded once
+template <typename T>
+__device__ __forceinline__ void store_row4(T* p, const float (&v)[4], int n) {
+    T o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = (T)v[i];
+    if (n >= 4) { __builtin_memcpy(p, o, sizeof(o)); return; }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < n) p[i] = o[i];
+}
+__device__ __forceinline__ void store_f32x4(void* base, int dtype, int64_t at, const float (&v)[4], int n) {
+    if (dtype == SPI_DTYPE_F32) store_row4((float*)base + at, v, n);
+    else if (dtype == SPI_DTYPE_F16) store_row4((half_t*)base + at, v, n);
+    else store_row4((bf16_t*)base + at, v, n);
+}
 __device__ __forceinline__ int dtype_bytes(int dtype) { return dtype == SPI_DTYPE_F32 ? 4 : dtype == SPI_DTYPE_I8 ? 1 : 2; }
 
 // ---- rows in 8 bits: t = max|v| / 127, q = rint(v / t).  The quotients are IEEE divisions: a row gives the same integers wherever it is quantised.

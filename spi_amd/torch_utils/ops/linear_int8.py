@@ -13,15 +13,15 @@ from . import bias_act as _ba
 MAX_IN_FEATURES = 131071         # SPI_LINEAR_INT8_MAX_K: 127 * 127 * in_features stays below 2^31
 
 
-def _rows(x, name):
-    """[..., K] -> [rows, K] with a row stride of at least K and adjacent values"""
+def _rows(x):
+    """[..., K] -> [rows, K] with adjacent values, and rows that are K .. 2^22 values apart"""
     k = x.shape[-1]
     x = x.reshape(-1, k)
-    return x if (k == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or x.stride(0) >= k) else x.contiguous()
+    return x if (k == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or k <= x.stride(0) <= 1 << 22) else x.contiguous()
 
 
 def _stride(x):
-    return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def quantize_rows(x):
@@ -38,7 +38,7 @@ def quantize_rows(x):
     with hip.on(device):
         q = torch.empty(x.shape[:-1] + (pitch,), device=device, dtype=torch.int8)
         scale = torch.empty(x.shape[:-1], device=device, dtype=torch.float32)
-        r = _rows(x.detach(), 'x')
+        r = _rows(x.detach())
         hip.call('spi_quantize_rows', r.data_ptr(), r.shape[0], k, _stride(r), hip.ROW_DTYPES[x.dtype], q.data_ptr(), pitch, scale.data_ptr(), hip.stream())
     return (q if pitch == k else q[..., :k]), scale
 
@@ -82,7 +82,7 @@ def linear_int8(x, weight_q, weight_scale, bias=None, x_scale=None, act='linear'
     device = hip.same_device(x, weight_q, weight_scale, bias, x_scale)
     with hip.on(device):
         y = torch.empty(x.shape[:-1] + (n,), device=device, dtype=out_dtype)
-        r, w = _rows(x, 'x'), _rows(weight_q, 'weight_q')
+        r, w = _rows(x), _rows(weight_q)
         m = r.shape[0]
         if m == 0:
             return y
