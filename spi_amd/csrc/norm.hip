@@ -63,12 +63,11 @@ __device__ __forceinline__ int64_t gate_at(const spi_norm_residual_desc& d, int6
     return d.gate_mode == GATE_FULL ? row * d.width : d.gate_mode == GATE_SAMPLE ? (int64_t)((unsigned)row / (unsigned)d.rows_per_sample) * d.width : 0;     // (rows < 2^31)
 }
 
-// mean and 1 / sqrt(mean square + eps) of the row held as x[NV][VEC]; columns outside the row are 0 in x and stay out of the centred sum
-template <int TPR, int NV, int VEC>
-__device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], const int (&left)[NV], int layer, float inv_width, float eps, float* red, int& phase, float& mean,
-                                          float& rstd) {
+// mean and 1 / sqrt(mean square + eps) of the row held as x[NV][VEC]; columns that are not this thread's are 0 in x and stay out of the centred sum
+template <int TPR, int NV, int VEC, bool LAYER>
+__device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], const int (&first)[NV], float inv_width, float eps, float* red, int& phase, float& mean, float& rstd) {
     mean = 0.f;
-    if (layer) {
+    if (LAYER) {
         float s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -78,113 +77,114 @@ __device__ __forceinline__ void row_stats(const float (&x)[NV][VEC], const int (
     }
     float q = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        float c[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float c = j < left[i] ? x[i][j] - mean : 0.f;
-            q = fmaf(c, c, q);
-        }
+        for (int j = 0; j < VEC; ++j) c[j] = x[i][j] - mean;
+        if (LAYER) mask_first(c, first[i], 0.f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) q = fmaf(c[j], c[j], q);
+    }
     rstd = 1.f / sqrtf(row_sum<TPR>(q, red, phase) * inv_width + eps);
 }
 
-template <typename T, int TPR, int NV>
+// One row in TPR threads, NV chunks of VEC values each.
+template <typename T, int VEC, int TPR, int NV, bool LAYER>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(const NormArgs a) {
-    constexpr int VEC = Chunk<T>::N, THREADS = TPR > 256 ? TPR : 256, G = THREADS / TPR;
+    constexpr int THREADS = TPR > 256 ? TPR : 256, G = THREADS / TPR;
     __shared__ float red[32];
     const spi_norm_residual_desc& d = a.d;
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * G + threadIdx.x / TPR;
-    const bool live = row < d.rows;                                            // (a dead row still meets every barrier of its block)
-    const int64_t base = (live ? row : 0) * d.width;
-    int phase = 0, left[NV];
-    float s[NV][VEC], r[NV][VEC];
+    const int64_t row_at = (int64_t)blockIdx.x * G + threadIdx.x / TPR;
+    const bool live = row_at < d.rows;                                         // (a dead row meets every barrier of its block, with another row's values)
+    const int64_t row = live ? row_at : d.rows - 1, base = row * d.width, gbase = d.gate_mode ? gate_at(d, row) : 0;
+    int phase = 0, at[NV], first[NV];
+    // (the gate and the weights are read where they are used: read ahead, or held for several rows, they cost so many registers that fewer rows are under way --
+    //  4 x 4096 x 2048 bf16: 60 us as it is, 79 and 68 us)
+    Chunk<T, VEC> hc[NV], rc[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c0 = (t + i * TPR) * VEC;
-        left[i] = live ? d.width - c0 : 0;
-        const Chunk<T> hc = load_chunk((const T*)d.h + base + c0, left[i]);
-        const Chunk<T> rc = load_chunk((const T*)d.residual + base + c0, left[i]);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) { s[i][j] = (float)hc.v[j]; r[i][j] = (float)rc.v[j]; }
+        const Columns c = columns<VEC>(t + i * TPR, d.width);
+        at[i] = c.start;
+        first[i] = c.first;
+        hc[i] = load_all<T, VEC>((const T*)d.h + base + c.start);
+        rc[i] = load_all<T, VEC>((const T*)d.residual + base + c.start);
     }
+    float s[NV][VEC];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) widen(hc[i], first[i], s[i]);
     float m1 = 0.f, r1 = 1.f;
-    if (d.after) row_stats<TPR, NV, VEC>(s, left, d.layer, a.inv_width, d.eps, red, phase, m1, r1);
-    const int64_t gbase = d.gate_mode ? gate_at(d, live ? row : 0) : 0;
+    if (d.after) row_stats<TPR, NV, VEC, LAYER>(s, first, a.inv_width, d.eps, red, phase, m1, r1);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c0 = (t + i * TPR) * VEC;
-        float w[VEC];
+        float w[VEC], r[VEC];
         if (d.after) {
-            load_f32(d.post_weight, d.weight_dtype, c0, left[i], w);
+            load_f32(d.post_weight, d.weight_dtype, at[i], w);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s[i][j] = (s[i][j] - m1) * r1 * w[j];
+            for (int j = 0; j < VEC; ++j) s[i][j] = (s[i][j] - (LAYER ? m1 : 0.f)) * r1 * w[j];
             if (d.post_bias) {
-                load_f32(d.post_bias, d.weight_dtype, c0, left[i], w);
+                load_f32(d.post_bias, d.weight_dtype, at[i], w);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) s[i][j] += w[j];
             }
         }
         if (d.gate_mode) {
-            load_f32(d.gate, d.gate_dtype, gbase + c0, left[i], w);
+            load_f32(d.gate, d.gate_dtype, gbase + at[i], w);
+            if (d.gate_act != SPI_ACT_LINEAR)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s[i][j] *= gate_value(d.gate_act, w[j]);
-        }
-        Chunk<T> out;
+                for (int j = 0; j < VEC; ++j) w[j] = gate_value(d.gate_act, w[j]);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            s[i][j] = j < left[i] ? r[i][j] + d.scale * s[i][j] : 0.f;
-            out.v[j] = (T)s[i][j];
+            for (int j = 0; j < VEC; ++j) s[i][j] *= w[j];
         }
-        store_chunk((T*)d.stream_out + base + c0, out, left[i]);
+        widen(rc[i], 0, r);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s[i][j] = fmaf(d.scale, s[i][j], r[j]);
+        mask_first(s[i], first[i], 0.f);
+        if (live && first[i] < VEC) store_columns((T*)d.stream_out + base + at[i], s[i], first[i]);
     }
     float m2 = 0.f, r2 = 1.f;
     if (d.before) {
-        row_stats<TPR, NV, VEC>(s, left, d.layer, a.inv_width, d.eps, red, phase, m2, r2);
+        row_stats<TPR, NV, VEC, LAYER>(s, first, a.inv_width, d.eps, red, phase, m2, r2);
         float amax = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c0 = (t + i * TPR) * VEC;
             float w[VEC];
-            load_f32(d.pre_weight, d.weight_dtype, c0, left[i], w);
+            load_f32(d.pre_weight, d.weight_dtype, at[i], w);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s[i][j] = (s[i][j] - m2) * r2 * w[j];
+            for (int j = 0; j < VEC; ++j) s[i][j] = (s[i][j] - (LAYER ? m2 : 0.f)) * r2 * w[j];
             if (d.pre_bias) {
-                load_f32(d.pre_bias, d.weight_dtype, c0, left[i], w);
+                load_f32(d.pre_bias, d.weight_dtype, at[i], w);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) s[i][j] += w[j];
             }
             if (d.q) {
+                mask_first(s[i], first[i], 0.f);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, j < left[i] ? abs_or_inf(s[i][j]) : 0.f);
-            } else {
-                Chunk<T> out;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) out.v[j] = (T)s[i][j];
-                store_chunk((T*)d.normed + base + c0, out, left[i]);
-            }
+                for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, abs_or_inf(s[i][j]));
+            } else if (live && first[i] < VEC) store_columns((T*)d.normed + base + at[i], s[i], first[i]);
         }
         if (d.q) {
             const float scale = row_scale(row_max<TPR>(amax, red, phase));
-            if (live && t == 0) d.q_scale[row] = scale;
+            int8_t* q = d.q + row * d.q_stride;
+            if (live) {
+                if (t == 0) d.q_scale[row] = scale;
+                if (t < d.q_stride - d.width) q[d.width + t] = 0;              // the padding (less than 16 bytes)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int c0 = (t + i * TPR) * VEC;
-                int8_t* p = d.q + (live ? row : 0) * d.q_stride + c0;          // (the padding behind the row is written as 0)
-                int8_t v[VEC];
+                for (int i = 0; i < NV; ++i) {
+                    Chunk<int8_t, VEC> v;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = j < left[i] ? (int8_t)quantize_value(s[i][j], scale) : (int8_t)0;
-                const int room = live ? (int)d.q_stride - c0 : 0;
-                if (room >= VEC) __builtin_memcpy(p, v, VEC);
-                else {
+                    for (int j = 0; j < VEC; ++j) v.v[j] = (int8_t)quantize_value(s[i][j], scale);
+                    if (first[i] <= 0) __builtin_memcpy(q + at[i], &v, VEC);
+                    else if (first[i] < VEC)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) if (j < room) p[j] = v[j];
+                        for (int j = 0; j < VEC; ++j) if (j >= first[i]) q[at[i] + j] = v.v[j];
                 }
             }
         }
     }
     if (d.stats && live && t == 0) {
-        float* p = d.stats + row * 4;
-        p[0] = m1; p[1] = r1; p[2] = m2; p[3] = r2;
+        const f32x4_t v = {m1, r1, m2, r2};
+        *reinterpret_cast<f32x4_t*>(d.stats + row * 4) = v;
     }
 }
 
@@ -201,29 +201,61 @@ enum { SUM_POST_W = 0, SUM_POST_B, SUM_PRE_W, SUM_PRE_B, N_SUMS, SUM_GATE = N_SU
 struct NormBwdArgs {
     spi_norm_residual_desc d;
     float inv_width;
-    int64_t nseg, seg_rows, segs_per_sample;           // rows of a segment; segments of one sample (the whole batch is one sample unless the gate is per sample)
+    int64_t nseg, segs_per_sample;                     // segments of one sample (the whole batch is one sample unless the gate is per sample)
     int64_t sample_rows;
     float* part;                                       // [grid][sums in use][width], then the gate's [nseg][width]
     float* gate_part;                                  // NULL: segments write d_gate themselves
     int slot[N_SUMS], slots;
 };
 
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(BT) norm_bwd_kernel(const NormBwdArgs a) {
-    constexpr int VEC = Chunk<T>::N, G = BT / TPR;
+// two sums over a row's threads behind one barrier
+template <int TPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int& phase) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (TPR > 64) {
+        constexpr int W = TPR / 64;
+        const int wave = threadIdx.x >> 6, first = wave / W * W;
+        float* r = red + (phase & 1) * 32;
+        ++phase;
+        if ((threadIdx.x & 63) == 0) { r[wave] = a; r[16 + wave] = b; }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) { a += r[first + i]; b += r[16 + first + i]; }
+    }
+}
+
+// Bound by HBM (h, residual, ds, dy in; d_h, d_residual out) as far as enough of it is under way: a block holds few rows, so the rows of the next two turns are on their way
+// while one is worked on.  With one row ahead a CU has 32 KB under way and 4 x 4096 x 2048 bf16 takes 139 us (2.9 TB/s), with or without the sums between the threads.
+template <typename T, int VEC, int TPR, int NV, bool LAYER>
+__global__ void __launch_bounds__(TPR > BT ? TPR : BT, TPR > BT ? 4 : sizeof(T) == 4 && NV == 1 ? 3 : 2) norm_bwd_kernel(const NormBwdArgs a) {
+    constexpr int G = TPR > BT ? 1 : BT / TPR;
+    constexpr bool AHEAD = NV == 1;                    // the next row is on its way (wide rows leave no registers for it)
+    typedef Chunk<T, VEC> Values;
     __shared__ float red[64];
     __shared__ float stage[G > 1 ? G * TPR * NV * VEC : 1];
     const spi_norm_residual_desc& d = a.d;
     const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
+    const bool full = d.gate_mode == GATE_FULL, bent = d.gate_act != SPI_ACT_LINEAR;
     int phase = 0;
-    float acc[N_SUMS + 1][NV][VEC];
+    float acc[N_SUMS + 1][NV][VEC], pw[NV][VEC], qw[NV][VEC], ga[NV][VEC];
+    int at[NV], first[NV];                             // this thread's columns
 #pragma unroll
-    for (int k = 0; k <= N_SUMS; ++k)
+    for (int i = 0; i < NV; ++i) {
+        const Columns c = columns<VEC>(t + i * TPR, d.width);
+        at[i] = c.start;
+        first[i] = c.first;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int j = 0; j < VEC; ++j) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[k][i][j] = 0.f;
-    // sum of acc[k] over the block's row groups, in every thread of group 0
+            for (int k = 0; k <= N_SUMS; ++k) acc[k][i][j] = 0.f;
+            pw[i][j] = qw[i][j] = ga[i][j] = 1.f;
+        }
+        if (d.after) load_f32(d.post_weight, d.weight_dtype, at[i], pw[i]);
+        if (d.before) load_f32(d.pre_weight, d.weight_dtype, at[i], qw[i]);
+    }
+    // the sum of v over the block's row groups, in every thread of group 0
     auto over_groups = [&](float (&v)[NV][VEC]) {
         if constexpr (G > 1) {
             __syncthreads();
@@ -241,129 +273,156 @@ __global__ void __launch_bounds__(BT) norm_bwd_kernel(const NormBwdArgs a) {
         }
     };
     for (int64_t seg = blockIdx.x; seg < a.nseg; seg += gridDim.x) {
-        const int64_t sample = seg / a.segs_per_sample, row0 = sample * a.sample_rows + (seg % a.segs_per_sample) * a.seg_rows;
-        const int64_t row1 = min(min(row0 + a.seg_rows, (sample + 1) * a.sample_rows), d.rows);
-        for (int64_t rb = row0; rb < row1; rb += G) {
-            const int64_t row = rb + g;
+        // G rows at a time, all segments of a sample side by side: blocks that each kept to rows of their own would all be at the same place of a 128 KB stride, on few of
+        // the memory's channels (4 x 4096 x 2048 bf16: 142 us)
+        const int64_t sample = seg / a.segs_per_sample, row0 = sample * a.sample_rows + seg % a.segs_per_sample * G, row1 = (sample + 1) * a.sample_rows;
+        const int64_t stride = a.segs_per_sample * G;
+        if (d.gate_mode && !full) {
+            const int64_t gbase = gate_at(d, row0);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                load_f32(d.gate, d.gate_dtype, gbase + at[i], ga[i]);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) ga[i][j] = bent ? gate_value(d.gate_act, ga[i][j]) : ga[i][j];
+            }
+        }
+        struct Row { Values h[NV], r[NV], s[NV], y[NV]; Raw<VEC> g[NV]; f32x4_t st; } in;
+        auto fetch = [&](int64_t row) {
+            const int64_t from = row < row1 ? row : row0, base = from * d.width;
+            in.st = *reinterpret_cast<const f32x4_t*>(d.stats + from * 4);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                in.h[i] = load_all<T, VEC>((const T*)d.h + base + at[i]);
+                if (d.before) {
+                    in.r[i] = load_all<T, VEC>((const T*)d.residual + base + at[i]);
+                    in.y[i] = load_all<T, VEC>((const T*)d.d_normed + base + at[i]);
+                }
+                if (d.d_stream) in.s[i] = load_all<T, VEC>((const T*)d.d_stream + base + at[i]);
+                if (full) in.g[i] = load_raw<VEC>(d.gate, d.gate_dtype, base + at[i]);
+            }
+        };
+        if (AHEAD) fetch(row0 + g);
+        for (int64_t rb = row0; rb < row1; rb += stride) {
+            const int64_t row = rb + g, base = row * d.width;
             const bool live = row < row1;
-            const int64_t base = (live ? row : row0) * d.width;
-            const float* st = d.stats + (live ? row : row0) * 4;
-            const float m1 = st[0], r1 = st[1], m2 = st[2], r2 = st[3];
-            const int64_t gbase = d.gate_mode ? gate_at(d, live ? row : row0) : 0;
-            float hh[NV][VEC], z[NV][VEC], ga[NV][VEC], tt[NV][VEC], sh[NV][VEC], u[NV][VEC];
-            int left[NV];
+            if (!AHEAD) fetch(row);
+            // Columns of others, and all of a dead row, are taken as 0 (a dead row's statistics, too): their u, t and dz are 0 and add nothing to any sum; only the layer
+            // norm's means reach them.
+            const float m1 = live ? in.st[0] : 0.f, r1 = live ? in.st[1] : 0.f, m2 = live ? in.st[2] : 0.f, r2 = live ? in.st[3] : 0.f;
+            float hh[NV][VEC], z[NV][VEC], tt[NV][VEC], sh[NV][VEC], u[NV][VEC];
+            int skip[NV];
             float sum_us = 0.f, sum_u = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c0 = (t + i * TPR) * VEC;
-                left[i] = live ? d.width - c0 : 0;
-                const Chunk<T> hc = load_chunk((const T*)d.h + base + c0, left[i]);
-                Chunk<T> rc, dsc, dyc;
-                if (d.before) rc = load_chunk((const T*)d.residual + base + c0, left[i]);
-                if (d.d_stream) dsc = load_chunk((const T*)d.d_stream + base + c0, left[i]);
-                if (d.before) dyc = load_chunk((const T*)d.d_normed + base + c0, left[i]);
-                float w[VEC];
+                skip[i] = live ? first[i] : VEC;
+                float x[VEC];
+                widen(in.h[i], skip[i], x);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) { hh[i][j] = ((float)hc.v[j] - m1) * r1; z[i][j] = hh[i][j]; ga[i][j] = 1.f; }
-                if (d.after) {
-                    load_f32(d.post_weight, d.weight_dtype, c0, left[i], w);
+                for (int j = 0; j < VEC; ++j) { hh[i][j] = (x[j] - (LAYER ? m1 : 0.f)) * r1; z[i][j] = hh[i][j] * pw[i][j]; }
+                if (d.post_bias) {
+                    float w[VEC];
+                    load_f32(d.post_bias, d.weight_dtype, at[i], w);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) z[i][j] *= w[j];
-                    if (d.post_bias) {
-                        load_f32(d.post_bias, d.weight_dtype, c0, left[i], w);
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) z[i][j] += w[j];
-                    }
+                    for (int j = 0; j < VEC; ++j) z[i][j] += w[j];
                 }
-                if (d.gate_mode) {
-                    load_f32(d.gate, d.gate_dtype, gbase + c0, left[i], w);
+                if (full) {
+                    widen<VEC>(in.g[i], d.gate_dtype, ga[i]);
+                    if (bent)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) ga[i][j] = gate_value(d.gate_act, w[j]);
+                        for (int j = 0; j < VEC; ++j) ga[i][j] = gate_value(d.gate_act, ga[i][j]);
                 }
+                if (d.d_stream) widen(in.s[i], skip[i], tt[i]);
+                else
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) tt[i][j] = d.d_stream && j < left[i] ? (float)dsc.v[j] : 0.f;
+                    for (int j = 0; j < VEC; ++j) tt[i][j] = 0.f;
                 if (d.before) {
-                    load_f32(d.pre_weight, d.weight_dtype, c0, left[i], w);
+                    float dy[VEC];
+                    widen(in.r[i], skip[i], x);
+                    widen(in.y[i], skip[i], dy);
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
-                        const float dy = j < left[i] ? (float)dyc.v[j] : 0.f;
-                        sh[i][j] = j < left[i] ? ((float)rc.v[j] + d.scale * ga[i][j] * z[i][j] - m2) * r2 : 0.f;
-                        acc[SUM_PRE_W][i][j] = fmaf(dy, sh[i][j], acc[SUM_PRE_W][i][j]);
-                        acc[SUM_PRE_B][i][j] += dy;
-                        u[i][j] = dy * w[j];
+                        sh[i][j] = (fmaf(d.scale * ga[i][j], z[i][j], x[j]) - (LAYER ? m2 : 0.f)) * r2;
+                        acc[SUM_PRE_W][i][j] = fmaf(dy[j], sh[i][j], acc[SUM_PRE_W][i][j]);
+                        u[i][j] = dy[j] * qw[i][j];
                         sum_us = fmaf(u[i][j], sh[i][j], sum_us);
-                        sum_u += u[i][j];
+                        if (LAYER) sum_u += u[i][j];
                     }
+                    if (d.d_pre_bias)
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) acc[SUM_PRE_B][i][j] += dy[j];
                 }
             }
+            if (AHEAD && rb + stride < row1) fetch(row + stride);      // (the same for the whole block)
             if (d.before) {
-                sum_us = row_sum<TPR>(sum_us, red, phase) * a.inv_width;
-                sum_u = d.layer ? row_sum<TPR>(sum_u, red, phase) * a.inv_width : 0.f;
+                if (LAYER) row_sum2<TPR>(sum_us, sum_u, red, phase);
+                else sum_us = row_sum<TPR>(sum_us, red, phase);
+                sum_us *= a.inv_width;
+                sum_u *= a.inv_width;
 #pragma unroll
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) tt[i][j] += j < left[i] ? r2 * (u[i][j] - sh[i][j] * sum_us - sum_u) : 0.f;
+                    for (int j = 0; j < VEC; ++j) {
+                        if (LAYER) tt[i][j] += j >= skip[i] ? r2 * (fmaf(-sh[i][j], sum_us, u[i][j]) - sum_u) : 0.f;
+                        else tt[i][j] = fmaf(r2, fmaf(-sh[i][j], sum_us, u[i][j]), tt[i][j]);
+                    }
             }
             float sum_vh = 0.f, sum_v = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c0 = (t + i * TPR) * VEC;
-                Chunk<T> out;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) out.v[j] = (T)tt[i][j];
-                if (d.d_residual) store_chunk((T*)d.d_residual + base + c0, out, left[i]);
-                float w[VEC];
-                if (d.after) load_f32(d.post_weight, d.weight_dtype, c0, left[i], w);
-                float dg[VEC];
+                if (d.d_residual && skip[i] < VEC) store_columns((T*)d.d_residual + base + at[i], tt[i], skip[i]);
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    dg[j] = j < left[i] ? gate_slope(d.gate_act, ga[i][j]) * d.scale * z[i][j] * tt[i][j] : 0.f;
-                    const float dz = d.scale * ga[i][j] * tt[i][j];
+                    tt[i][j] *= d.scale;
+                    const float dz = ga[i][j] * tt[i][j];
                     u[i][j] = dz;
                     if (d.after) {
-                        const float hv = j < left[i] ? hh[i][j] : 0.f;
-                        acc[SUM_POST_W][i][j] = fmaf(dz, hv, acc[SUM_POST_W][i][j]);
-                        acc[SUM_POST_B][i][j] += dz;
-                        u[i][j] = dz * w[j];
-                        sum_vh = fmaf(u[i][j], hv, sum_vh);
-                        sum_v += u[i][j];
+                        acc[SUM_POST_W][i][j] = fmaf(dz, hh[i][j], acc[SUM_POST_W][i][j]);
+                        u[i][j] = dz * pw[i][j];
+                        sum_vh = fmaf(u[i][j], hh[i][j], sum_vh);
+                        if (LAYER) sum_v += u[i][j];
                     }
                 }
-                if (d.gate_mode == GATE_FULL) {
-                    if (d.d_gate)
+                if (d.d_post_bias)
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) if (j < left[i]) store_f32(d.d_gate, d.gate_dtype, base + c0 + j, dg[j]);
-                } else if (d.gate_mode) {
+                    for (int j = 0; j < VEC; ++j) acc[SUM_POST_B][i][j] = fmaf(ga[i][j], tt[i][j], acc[SUM_POST_B][i][j]);
+                if (d.d_gate) {
+                    float dg[VEC];
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) acc[SUM_GATE][i][j] += dg[j];
+                    for (int j = 0; j < VEC; ++j) dg[j] = z[i][j] * tt[i][j];
+                    if (bent)
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) dg[j] *= gate_slope(d.gate_act, ga[i][j]);
+                    if (full) {
+                        if (skip[i] < VEC) store_columns<VEC>(d.d_gate, d.gate_dtype, base + at[i], dg, skip[i]);
+                    } else
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) acc[SUM_GATE][i][j] += dg[j];
                 }
             }
             if (d.after) {
-                sum_vh = row_sum<TPR>(sum_vh, red, phase) * a.inv_width;
-                sum_v = d.layer ? row_sum<TPR>(sum_v, red, phase) * a.inv_width : 0.f;
+                if (LAYER) row_sum2<TPR>(sum_vh, sum_v, red, phase);
+                else sum_vh = row_sum<TPR>(sum_vh, red, phase);
+                sum_vh *= a.inv_width;
+                sum_v *= a.inv_width;
             }
             if (d.d_h)
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    const int c0 = (t + i * TPR) * VEC;
-                    Chunk<T> out;
+                    if (d.after)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) out.v[j] = (T)(d.after ? r1 * (u[i][j] - hh[i][j] * sum_vh - sum_v) : u[i][j]);
-                    store_chunk((T*)d.d_h + base + c0, out, left[i]);
+                        for (int j = 0; j < VEC; ++j) u[i][j] = r1 * (fmaf(-hh[i][j], sum_vh, u[i][j]) - sum_v);
+                    if (skip[i] < VEC) store_columns((T*)d.d_h + base + at[i], u[i], skip[i]);
                 }
         }
         if (d.d_gate && (d.gate_mode == GATE_CHANNEL || d.gate_mode == GATE_SAMPLE)) {
             over_groups(acc[SUM_GATE]);
             if (g == 0)
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const int c = (t + i * TPR) * VEC + j;
-                        if (c >= d.width) continue;
-                        if (a.gate_part) a.gate_part[seg * d.width + c] = acc[SUM_GATE][i][j];
-                        else store_f32(d.d_gate, d.gate_dtype, sample * d.width + c, acc[SUM_GATE][i][j]);
-                    }
+                for (int i = 0; i < NV; ++i) {
+                    if (first[i] >= VEC) continue;
+                    if (a.gate_part) store_columns(a.gate_part + seg * d.width + at[i], acc[SUM_GATE][i], first[i]);
+                    else store_columns<VEC>(d.d_gate, d.gate_dtype, sample * d.width + at[i], acc[SUM_GATE][i], first[i]);
+                }
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -377,47 +436,48 @@ __global__ void __launch_bounds__(BT) norm_bwd_kernel(const NormBwdArgs a) {
         if (g == 0)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int c = (t + i * TPR) * VEC + j;
-                    if (c < d.width) a.part[((int64_t)blockIdx.x * a.slots + a.slot[k]) * d.width + c] = acc[k][i][j];
-                }
+                if (first[i] < VEC) store_columns(a.part + ((int64_t)blockIdx.x * a.slots + a.slot[k]) * d.width + at[i], acc[k][i], first[i]);
     }
 }
 
-// out[v][c] = sum_p part[v * v_stride + p * p_stride + c], four rows of partial sums per column in flight, added in a fixed order
+// out[v][c] = sum_p part[v * v_stride + p * p_stride + c]: 16 chains of partial sums for each column, eight loads of each in flight, joined in a fixed order
 struct ReduceJob { const float* part; void* out; int dtype; int64_t v_stride, p_stride, parts, vectors; };
 struct ReduceArgs { ReduceJob job[N_SUMS + 1]; int64_t first[N_SUMS + 2]; int jobs, width, cols; };
-__global__ void __launch_bounds__(256) norm_bwd_reduce_kernel(const ReduceArgs a) {
-    __shared__ float s[4][64];
+__global__ void __launch_bounds__(1024) norm_bwd_reduce_kernel(const ReduceArgs a) {
+    __shared__ float s[16][64];
     int j = 0;
     while (j + 1 < a.jobs && (int64_t)blockIdx.x >= a.first[j + 1]) ++j;
     const ReduceJob& q = a.job[j];
     const int64_t b = blockIdx.x - a.first[j], v = b / a.cols;
     const int c = (int)(b % a.cols) * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
     float x = 0.f;
-    if (c < a.width)
-        for (int64_t p = r; p < q.parts; p += 4) x += q.part[v * q.v_stride + p * q.p_stride + c];
+    if (c < a.width) {
+        const float* p = q.part + v * q.v_stride + c;
+#pragma unroll 8
+        for (int64_t i = r; i < q.parts; i += 16) x += p[i * q.p_stride];
+    }
     s[r][threadIdx.x & 63] = x;
     __syncthreads();
-    if (r == 0 && c < a.width) store_f32(q.out, q.dtype, v * a.width + c, (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]));
+    if (r || c >= a.width) return;
+    for (int i = 1; i < 16; ++i) x += s[i][threadIdx.x];
+    store_f32(q.out, q.dtype, v * a.width + c, x);
 }
 
-struct BwdPlan { int64_t nseg, seg_rows, segs_per_sample, sample_rows, samples; int grid, tpr; bool gate_reduce; };
+struct BwdPlan { int64_t nseg, segs_per_sample, sample_rows, samples; int grid, tpr; bool wide, gate_reduce; };
 
-// threads of a row in the backward: eight values each, sixteen over 4096 (so that five column sums of a thread's columns stay in its registers)
-int bwd_tpr(int width) { return width <= 512 ? 64 : width <= 2048 ? 256 : 512; }
+// threads of a row in the backward
+int bwd_tpr(int chunks, bool wide) { return chunks <= 64 ? 64 : chunks <= 256 ? 256 : chunks <= 512 || wide ? 512 : 1024; }
 
 BwdPlan bwd_plan(const spi_norm_residual_desc& d) {
     BwdPlan p;
-    p.tpr = bwd_tpr(d.width);
-    const int G = BT / p.tpr;
+    const int chunks = (int)ceil_div64(d.width, d.dtype == SPI_DTYPE_F32 ? 4 : 8);
+    p.wide = d.width > 4096;                           // sixteen values a thread
+    p.tpr = bwd_tpr(chunks, p.wide);
+    const int G = std::max(1, BT / p.tpr);
     p.sample_rows = d.gate_mode == GATE_SAMPLE ? d.rows_per_sample : d.rows;
     p.samples = p.sample_rows ? d.rows / p.sample_rows : 0;
     const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, p.samples));              // segments of a sample: two blocks for every CU
     p.segs_per_sample = std::max<int64_t>(1, std::min(want, ceil_div64(p.sample_rows, G)));
-    p.seg_rows = ceil_div64(ceil_div64(p.sample_rows, p.segs_per_sample), G) * G;
-    p.segs_per_sample = std::max<int64_t>(1, ceil_div64(p.sample_rows, p.seg_rows ? p.seg_rows : 1));
     p.nseg = p.samples * p.segs_per_sample;
     p.grid = (int)std::min<int64_t>(p.nseg, 512);
     p.gate_reduce = d.d_gate && (d.gate_mode == GATE_CHANNEL || d.gate_mode == GATE_SAMPLE) && p.segs_per_sample > 1;
@@ -451,30 +511,42 @@ int check_desc(const spi_norm_residual_desc* d, const char* who) {
     return SPI_OK;
 }
 
-template <typename T, int TPR, int NV>
+template <typename T, int VEC, int TPR, int NV>
 void launch_fwd(const NormArgs& a, hipStream_t st) {
     constexpr int THREADS = TPR > 256 ? TPR : 256;
-    hipLaunchKernelGGL((norm_fwd_kernel<T, TPR, NV>), dim3((unsigned)ceil_div64(a.d.rows, THREADS / TPR)), dim3(THREADS), 0, st, a);
+    const dim3 grid((unsigned)ceil_div64(a.d.rows, THREADS / TPR));
+    if (a.d.layer) hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, TPR, NV, true>), grid, dim3(THREADS), 0, st, a);
+    else hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, TPR, NV, false>), grid, dim3(THREADS), 0, st, a);
 }
 template <typename T>
 void dispatch_fwd(const NormArgs& a, hipStream_t st) {
-    const int chunks = (int)ceil_div64(a.d.width, Chunk<T>::N);
-    if (chunks <= 64) launch_fwd<T, 64, 1>(a, st);
-    else if (chunks <= 128) launch_fwd<T, 64, 2>(a, st);
-    else if (chunks <= 256) launch_fwd<T, 256, 1>(a, st);
-    else if (chunks <= 512) launch_fwd<T, 256, 2>(a, st);
-    else if (chunks <= 1024) launch_fwd<T, 256, 4>(a, st);
-    else if (chunks <= 2048) launch_fwd<T, 1024, 2>(a, st);
-    else if (sizeof(T) < 4 || chunks <= 4096) launch_fwd<T, 1024, 4>(a, st);       // (SPI_NORM_MAX_WIDTH is 4096 chunks of eight)
-    else if constexpr (sizeof(T) == 4) launch_fwd<T, 1024, 8>(a, st);
+    constexpr int N = Chunk<T>::N;
+    const int chunks = (int)ceil_div64(a.d.width, N);
+    if (a.d.width < N) launch_fwd<T, 1, 64, 1>(a, st);
+    else if (chunks <= 64) launch_fwd<T, N, 64, 1>(a, st);
+    else if (chunks <= 128) launch_fwd<T, N, 64, 2>(a, st);
+    else if (chunks <= 256) launch_fwd<T, N, 256, 1>(a, st);
+    else if (chunks <= 512) launch_fwd<T, N, 256, 2>(a, st);
+    else if (chunks <= 1024) launch_fwd<T, N, 256, 4>(a, st);
+    else if (chunks <= 2048) launch_fwd<T, N, 1024, 2>(a, st);
+    else if (sizeof(T) < 4 || chunks <= 4096) launch_fwd<T, N, 1024, 4>(a, st);       // (SPI_NORM_MAX_WIDTH is 4096 chunks of eight)
+    else if constexpr (sizeof(T) == 4) launch_fwd<T, N, 1024, 8>(a, st);
+}
+template <typename T, int VEC, int TPR, int NV>
+void launch_bwd(const NormBwdArgs& a, int grid, hipStream_t st) {
+    const dim3 block(TPR > BT ? TPR : BT);
+    if (a.d.layer) hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, TPR, NV, true>), dim3(grid), block, 0, st, a);
+    else hipLaunchKernelGGL((norm_bwd_kernel<T, VEC, TPR, NV, false>), dim3(grid), block, 0, st, a);
 }
 template <typename T>
 void dispatch_bwd(const NormBwdArgs& a, const BwdPlan& p, hipStream_t st) {
-    constexpr int NV = 8 / Chunk<T>::N;
-    if (p.tpr == 64) hipLaunchKernelGGL((norm_bwd_kernel<T, 64, NV>), dim3(p.grid), dim3(BT), 0, st, a);
-    else if (p.tpr == 256) hipLaunchKernelGGL((norm_bwd_kernel<T, 256, NV>), dim3(p.grid), dim3(BT), 0, st, a);
-    else if (a.d.width <= 4096) hipLaunchKernelGGL((norm_bwd_kernel<T, 512, NV>), dim3(p.grid), dim3(BT), 0, st, a);
-    else hipLaunchKernelGGL((norm_bwd_kernel<T, 512, 2 * NV>), dim3(p.grid), dim3(BT), 0, st, a);
+    constexpr int N = Chunk<T>::N;
+    if (a.d.width < N) launch_bwd<T, 1, 64, 1>(a, p.grid, st);
+    else if (p.wide) launch_bwd<T, N, 512, 16 / N>(a, p.grid, st);
+    else if (p.tpr == 64) launch_bwd<T, N, 64, 1>(a, p.grid, st);
+    else if (p.tpr == 256) launch_bwd<T, N, 256, 1>(a, p.grid, st);
+    else if (p.tpr == 512) launch_bwd<T, N, 512, 1>(a, p.grid, st);
+    else if constexpr (sizeof(T) == 4) launch_bwd<T, N, 1024, 1>(a, p.grid, st);
 }
 
 }  // namespace
@@ -514,7 +586,7 @@ extern "C" int spi_norm_residual_bwd(const spi_norm_residual_desc* d, spi_stream
     NormBwdArgs a;
     a.d = *d;
     a.inv_width = 1.f / (float)d->width;
-    a.nseg = p.nseg; a.seg_rows = p.seg_rows; a.segs_per_sample = p.segs_per_sample; a.sample_rows = p.sample_rows;
+    a.nseg = p.nseg; a.segs_per_sample = p.segs_per_sample; a.sample_rows = p.sample_rows;
     a.slots = sums_in_use(*d, a.slot);
     a.part = (float*)d->workspace;
     a.gate_part = p.gate_reduce ? a.part + (int64_t)p.grid * a.slots * d->width : nullptr;
@@ -535,7 +607,7 @@ extern "C" int spi_norm_residual_bwd(const spi_norm_residual_desc* d, spi_stream
         if (outs[k]) add(a.part + (int64_t)a.slot[k] * d->width, outs[k], d->weight_dtype, 0, (int64_t)a.slots * d->width, p.grid, 1);
     if (p.gate_reduce) add(a.gate_part, d->d_gate, d->gate_dtype, p.segs_per_sample * d->width, d->width, p.segs_per_sample, p.samples);
     if (r.jobs) {
-        hipLaunchKernelGGL(norm_bwd_reduce_kernel, dim3((unsigned)r.first[r.jobs]), dim3(256), 0, st, r);
+        hipLaunchKernelGGL(norm_bwd_reduce_kernel, dim3((unsigned)r.first[r.jobs]), dim3(1024), 0, st, r);
         SPI_LAUNCH_CHECK("spi_norm_residual_bwd (sums)");
     }
     return SPI_OK;

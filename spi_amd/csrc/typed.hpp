@@ -9,49 +9,77 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_acc __attribute__((ext_vector_type(16)));
 typedef int i32x16_acc __attribute__((ext_vector_type(16)));
 
-template <typename T> struct Chunk {                            // 16 bytes of a row: 4 floats, 8 halves, 16 bytes
-    static constexpr int N = 16 / (int)sizeof(T);
+// N neighbours of a row; `n` of them valid at p (any alignment of T), the others 0.  All of them are one load of up to 16 bytes: gfx950 takes it at the alignment of T.
+template <typename T, int N_ = 16 / (int)sizeof(T)>
+struct Chunk {
+    static constexpr int N = N_;
     T v[N];
 };
-
-// `n` valid values at p (any alignment of T), the others 0.  A whole chunk is one 16-byte load: gfx950 takes it at the alignment of T.
-template <typename T>
-__device__ __forceinline__ Chunk<T> load_chunk(const T* __restrict__ p, int n) {
-    Chunk<T> c;
-    if (n >= Chunk<T>::N) { __builtin_memcpy(&c, p, 16); return c; }
+template <typename T, int N = 16 / (int)sizeof(T)>
+__device__ __forceinline__ Chunk<T, N> load_chunk(const T* __restrict__ p, int n) {
+    Chunk<T, N> c;
+    if (n >= N) { __builtin_memcpy(&c, p, sizeof(c)); return c; }
 #pragma unroll
-    for (int i = 0; i < Chunk<T>::N; ++i) c.v[i] = i < n ? p[i] : (T)0;
+    for (int i = 0; i < N; ++i) c.v[i] = i < n ? p[i] : (T)0;
     return c;
 }
-template <typename T>
-__device__ __forceinline__ void store_chunk(T* __restrict__ p, const Chunk<T>& c, int n) {
-    if (n >= Chunk<T>::N) { __builtin_memcpy(p, &c, 16); return; }
+template <typename T, int N>
+__device__ __forceinline__ void store_chunk(T* __restrict__ p, const Chunk<T, N>& c, int n) {
+    if (n >= N) { __builtin_memcpy(p, &c, sizeof(c)); return; }
 #pragma unroll
-    for (int i = 0; i < Chunk<T>::N; ++i) if (i < n) p[i] = c.v[i];
+    for (int i = 0; i < N; ++i) if (i < n) p[i] = c.v[i];
 }
-// N values of a row vector whose type is known at run time only (a wave-uniform branch), widened to fp32
+// A thread's N columns of a row, for loads that ask nothing: N neighbours from `start` on, of which those before `first` are not this thread's (they belong to the chunk before
+// it, or -- first >= N -- all of them to others).  A load under a condition would be closed by a wait for it; these stay under way until their values are used.
+struct Columns { int start, first; };
 template <int N>
-__device__ __forceinline__ void load_f32(const void* base, int dtype, int64_t at, int n, float (&out)[N]) {
+__device__ __forceinline__ Columns columns(int chunk, int width) {             // width >= N
+    const int c0 = chunk * N, start = min(c0, width - N);
+    return Columns{start, c0 - start};
+}
+template <typename T, int N>
+__device__ __forceinline__ Chunk<T, N> load_all(const T* __restrict__ p) {
+    Chunk<T, N> c;
+    __builtin_memcpy(&c, p, sizeof(c));
+    return c;
+}
+template <int N, typename V>
+__device__ __forceinline__ void mask_first(float (&v)[N], int first, V other) {
+    if (first > 0)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = j < first ? other : v[j];
+}
+template <typename T, int N>
+__device__ __forceinline__ void widen(const Chunk<T, N>& c, int first, float (&out)[N]) {       // 0 where the column is not this thread's
+#pragma unroll
+    for (int j = 0; j < N; ++j) out[j] = (float)c.v[j];
+    mask_first(out, first, 0.f);
+}
+// values of a type known at run time only (a wave-uniform branch): as they lie in memory, and widened to fp32
+template <int N> struct Raw { uint32_t v[N]; };
+template <int N>
+__device__ __forceinline__ Raw<N> load_raw(const void* base, int dtype, int64_t at) {
+    Raw<N> r;
+    if (dtype == SPI_DTYPE_F32) __builtin_memcpy(&r, (const uint32_t*)base + at, 4 * N);
+    else if constexpr (N > 1) __builtin_memcpy(&r, (const uint16_t*)base + at, 2 * N);
+    else r.v[0] = ((const uint16_t*)base)[at];
+    return r;
+}
+template <int N>
+__device__ __forceinline__ void widen(const Raw<N>& r, int dtype, float (&out)[N]) {
     if (dtype == SPI_DTYPE_F32) {
-        const float* p = (const float*)base + at;
 #pragma unroll
-        for (int i = 0; i < N; i += 4) {
-            const Chunk<float> c = load_chunk(p + i, n - i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[i + j] = c.v[j];
-        }
+        for (int i = 0; i < N; ++i) out[i] = __builtin_bit_cast(float, r.v[i]);
         return;
     }
-    const uint16_t* p = (const uint16_t*)base + at;
-    uint16_t v[N];
-    if (n >= N) __builtin_memcpy(v, p, 2 * N);
-    else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i < n ? p[i] : (uint16_t)0;
+    for (int i = 0; i < N; ++i) {
+        const uint16_t h = (uint16_t)(r.v[i / 2] >> (i % 2 * 16));
+        out[i] = dtype == SPI_DTYPE_F16 ? (float)__builtin_bit_cast(half_t, h) : __builtin_bit_cast(float, (uint32_t)h << 16);
     }
-#pragma unroll
-    for (int i = 0; i < N; ++i) out[i] = dtype == SPI_DTYPE_F16 ? (float)__builtin_bit_cast(half_t, v[i]) : __builtin_bit_cast(float, (uint32_t)v[i] << 16);
 }
+template <int N>
+__device__ __forceinline__ void load_f32(const void* base, int dtype, int64_t at, float (&out)[N]) { widen<N>(load_raw<N>(base, dtype, at), dtype, out); }
 __device__ __forceinline__ void store_f32(void* base, int dtype, int64_t at, float v) {          // one rounding, to nearest even
     if (dtype == SPI_DTYPE_F32) ((float*)base)[at] = v;
     else if (dtype == SPI_DTYPE_F16) ((half_t*)base)[at] = (half_t)v;
@@ -66,6 +94,22 @@ __device__ __forceinline__ void store_row4(T* p, const float (&v)[4], int n) {
     if (n >= 4) { __builtin_memcpy(p, o, sizeof(o)); return; }
 #pragma unroll
     for (int i = 0; i < 4; ++i) if (i < n) p[i] = o[i];
+}
+// a thread's columns, rounded once: all of them, or those from `first` on
+template <typename T, int N>
+__device__ __forceinline__ void store_columns(T* p, const float (&v)[N], int first) {
+    Chunk<T, N> c;
+#pragma unroll
+    for (int j = 0; j < N; ++j) c.v[j] = (T)v[j];
+    if (first <= 0) { __builtin_memcpy(p, &c, sizeof(c)); return; }
+#pragma unroll
+    for (int j = 0; j < N; ++j) if (j >= first) p[j] = c.v[j];
+}
+template <int N>
+__device__ __forceinline__ void store_columns(void* base, int dtype, int64_t at, const float (&v)[N], int first) {
+    if (dtype == SPI_DTYPE_F32) store_columns((float*)base + at, v, first);
+    else if (dtype == SPI_DTYPE_F16) store_columns((half_t*)base + at, v, first);
+    else store_columns((bf16_t*)base + at, v, first);
 }
 __device__ __forceinline__ void store_f32x4(void* base, int dtype, int64_t at, const float (&v)[4], int n) {
     if (dtype == SPI_DTYPE_F32) store_row4((float*)base + at, v, n);

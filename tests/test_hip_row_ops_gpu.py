@@ -204,6 +204,22 @@ def test_norm_rows_stand_alone():
     assert torch.isnan(scale[1:4]).all() and torch.isfinite(scale[[0, 4, 5]]).all() and scale[4] == 0 and not q[1:5].any()
 
 
+def test_norm_gradients_of_rows_with_nan():
+    """a NaN row spoils its own gradients and the sums over rows that it is part of, and no other sample's"""
+    i = norm_inputs((3, 5, 200), F32, 'rms', 'both', 'sample', False)
+    i['h'][0, 0, 7] = float('nan')                                  # (the first row: what rows that a block has too few of read their statistics from)
+    leaves = {k: v.clone().requires_grad_() for k, v in i.items() if v is not None}
+    s, y = run_norm({k: leaves.get(k) for k in i}, 0.1, 'rms', 'both', 1e-6, 'linear')
+    ds, dy = randn(gen(1), 3, 5, 200), randn(gen(2), 3, 5, 200)
+    got = dict(zip(leaves, torch.autograd.grad([s, y], list(leaves.values()), [ds, dy])))
+    clean = {k: (v[1:].clone() if v.ndim == 3 else v.clone()).requires_grad_() for k, v in i.items() if v is not None}
+    s, y = run_norm({k: clean.get(k) for k in i}, 0.1, 'rms', 'both', 1e-6, 'linear')
+    want = dict(zip(clean, torch.autograd.grad([s, y], list(clean.values()), [ds[1:], dy[1:]])))
+    for k in ('h', 'residual', 'gate'):
+        assert torch.isnan(got[k][0]).any() and torch.equal(got[k][1:], want[k]), k
+    assert torch.isfinite(got['h'][0, 1:]).all() and torch.isfinite(got['residual'][0, 1:]).all() and torch.isnan(got['pre_weight']).any()
+
+
 def test_norm_strides_empty_and_repeat():
     i = norm_inputs((8, 12, 64), BF16, 'layer', 'both', 'full', True)
     want = run_norm(i, 0.1, 'layer', 'both', 1e-6, 'linear')
