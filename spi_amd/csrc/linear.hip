@@ -101,19 +101,20 @@ __device__ __forceinline__ float int8_epilogue(const Int8Args& a, int acc, float
 }
 
 // Tiles of 256 x 256 (8 waves), 128 x 128 and 64 x 64 (4 waves).
-template <typename T, int SIZE, bool COLA, bool COLB, bool DMA>
-using Engine = TileEngine<T, SIZE, SIZE, 2, SIZE == 256 ? 4 : 2, COLA, COLB, DMA>;
+template <typename T, int SIZE, bool COLA, bool COLB, int LOAD>
+using Engine = TileEngine<T, SIZE, SIZE, 2, SIZE == 256 ? 4 : 2, COLA, COLB, LOAD>;
 
-template <int SIZE, bool DMA>
+template <int SIZE, int LOAD>
 __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) int8_tile_kernel(const Int8Args a, int rows, int cols) {
-    typedef Engine<int8_t, SIZE, false, false, DMA> E;
+    typedef Engine<int8_t, SIZE, false, false, LOAD> E;
     __shared__ __attribute__((aligned(1024))) char s0[E::STAGE], s1[E::STAGE];
     int row, col;
     band_order(xcd_run(blockIdx.x, gridDim.x), rows, cols, row, col);
     const int m0 = row * SIZE, n0 = col * SIZE, m = min(SIZE, a.M - m0), n = min(SIZE, a.N - n0);
     typename E::Accs acc = {};
-    const int64_t k = DMA ? (a.K + 15) / 16 * 16 : a.K;                        // (DMA: the padding of the quantised rows is 0, so that of the weights does not count)
-    const TileOperand A{(const char*)a.q + m0 * a.q_stride, a.q_stride, m * a.q_stride, k, m}, B{(const char*)a.w + n0 * a.w_stride, a.w_stride, n * a.w_stride, k, n};
+    const int64_t k = LOAD == LOAD_DMA ? (a.K + 15) / 16 * 16 : a.K;           // (LOAD_DMA: the padding of the quantised rows is 0, so that of the weights does not count)
+    const TileOperand A{(const char*)a.q + m0 * a.q_stride, a.q_stride, m * a.q_stride, k, m, (int64_t)(a.M - 1 - m0) * a.q_stride + a.K},
+        B{(const char*)a.w + n0 * a.w_stride, a.w_stride, n * a.w_stride, k, n, (int64_t)(a.N - 1 - n0) * a.w_stride + a.K};
     E::run(A, B, s0, s1, acc);
     E::each(acc, s0, s1, [&](int i, int j, i32x4_t v) {
         if (i >= m || j >= n) return;
@@ -126,53 +127,142 @@ __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) int8_tile_kernel(cons
     });
 }
 
-// One row in TPR threads, NV chunks each held in registers (NV = 0: a row of any length, read twice)
+// Up to 16 rows: 16 outputs a block, the summed axis over its four waves, whose weights go straight from memory to the matrix cores (v_mfma_i32_16x16x64_i8) -- all of a wave's
+// loads under way at once.  The rows wait in LDS: int8 rows as they are; up to four rows of floats are quantised by every block, each for itself (one launch fewer).
+// Bound by latency: 1 x 512 x 512 takes 9.6 us as a tile of 64 x 64 behind a launch that quantises, 14 x 2048 x 4096 (8 MB of weights) 11 us.
+constexpr int FEW = 16, FEW_FLOATS = 4, FEW_LDS = 60000;
+__host__ __device__ inline int few_pitch(int K) { return (K + 63) / 64 * 64 + 16; }
+
+template <typename T>
+__global__ void __launch_bounds__(256) int8_few_rows_kernel(const Int8Args a, const T* __restrict__ x, int64_t x_stride, int64_t w_bytes) {
+    extern __shared__ __attribute__((aligned(16))) char rows[];               // [M][few_pitch(K)]
+    __shared__ float scales[FEW], red[2][4];
+    __shared__ int part[4][FEW][FEW + 1];
+    constexpr int N = Chunk<T>::N;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pitch = few_pitch(a.K), n0 = blockIdx.x * FEW;
+    if constexpr (sizeof(T) == 1) {
+        const int whole = a.K / 16, rest = pitch / 16 - whole;
+#pragma unroll 4
+        for (int c = tid; c < a.M * whole; c += 256) {
+            const int m = c / whole, k = c % whole * 16;
+            *reinterpret_cast<i32x4_t*>(rows + m * pitch + k) = __builtin_bit_cast(i32x4_t, load_all<int8_t, 16>((const int8_t*)x + m * x_stride + k));
+        }
+        for (int c = tid; c < a.M * rest; c += 256) {
+            const int m = c / rest, k = (whole + c % rest) * 16;
+            *reinterpret_cast<i32x4_t*>(rows + m * pitch + k) = __builtin_bit_cast(i32x4_t, load_chunk((const int8_t*)x + m * x_stride + (k < a.K ? k : 0), a.K - k));
+        }
+        if (tid < a.M) scales[tid] = a.q_scale[tid];
+    } else {
+        for (int m = 0; m < a.M; ++m) {                                        // the row is read twice, the second time from the cache
+            const T* p = x + m * x_stride;
+            float amax = 0.f;
+            for (int k = tid * N; k < a.K; k += 256 * N) {
+                const Chunk<T> c = load_chunk(p + k, a.K - k);
+#pragma unroll
+                for (int j = 0; j < N; ++j) amax = fmaxf(amax, abs_or_inf((float)c.v[j]));
+            }
+            amax = wave_max(amax);
+            if (lane == 0) red[m & 1][wave] = amax;
+            __syncthreads();
+            const float scale = row_scale(fmaxf(fmaxf(red[m & 1][0], red[m & 1][1]), fmaxf(red[m & 1][2], red[m & 1][3])));
+            const float inverse = 1.f / scale;
+            if (tid == 0) scales[m] = scale;
+            for (int k = tid * N; k < pitch; k += 256 * N) {
+                const Chunk<T> c = load_chunk(p + (k < a.K ? k : 0), a.K - k);
+                float f[N];
+                widen(c, 0, f);
+                const Chunk<int8_t, N> q = quantize_values(f, scale, inverse);
+                __builtin_memcpy(rows + m * pitch + k, &q, N);
+            }
+        }
+    }
+    __syncthreads();
+    const int steps = (a.K + 63) / 64, from = steps * wave / 4, to = steps * (wave + 1) / 4, n = min(n0 + (lane & 15), a.N - 1), kg = (lane >> 4) * 16;
+    const int8_t* w = a.w + n * a.w_stride;
+    const int64_t room = w_bytes - n * a.w_stride;                             // a chunk that runs on behind the row reads what lies there, against zeros in the rows
+    const char* q = rows + min(lane & 15, a.M - 1) * pitch + kg;
+    typedef int i32x4_acc __attribute__((ext_vector_type(4)));
+    i32x4_acc acc = {0, 0, 0, 0};
+    int k = from;
+    const bool whole = to * 64 <= w_bytes - min(n0 + FEW - 1, a.N - 1) * a.w_stride;           // for the whole wave: a matrix instruction wants all its lanes
+    for (; whole && k + 8 <= to; k += 8) {
+        i32x4_t b[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = __builtin_bit_cast(i32x4_t, load_all<int8_t, 16>(w + (k + i) * 64 + kg));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4_t*>(q + (k + i) * 64), b[i], acc, 0, 0, 0);
+    }
+    for (; k < to; ++k) {
+        const int64_t left = room - (k * 64 + kg);
+        const i32x4_t b = __builtin_bit_cast(i32x4_t, load_chunk(w + (left > 0 ? k * 64 + kg : 0), (int)(left < 16 ? left : 16)));
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const i32x4_t*>(q + k * 64), b, acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) part[wave][(lane >> 4) * 4 + r][lane & 15] = acc[r];
+    __syncthreads();
+    const int m = tid >> 4, c = tid & 15;
+    if (m >= a.M || n0 + c >= a.N) return;
+    const int sum = part[0][m][c] + part[1][m][c] + part[2][m][c] + part[3][m][c];
+    store_f32(a.y, a.y_dtype, (int64_t)m * a.N + n0 + c, int8_epilogue(a, sum, scales[m], a.w_scale[n0 + c], a.bias ? a.bias[n0 + c] : 0.f));
+}
+
+// One row in TPR threads, NV chunks each held in registers; NV = 0: a row of any length, read twice.
+// 8192 x 4096 bf16: 30 us with loads under a condition, which are waited for one by one.
 template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t rows, int width, int64_t x_stride, int8_t* __restrict__ q, int64_t q_stride,
                                                             int q_room, float* __restrict__ scales) {
     constexpr int VEC = Chunk<T>::N, G = 256 / TPR;
     __shared__ float red[4];
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * G + threadIdx.x / TPR;
-    const bool live = row < rows;
-    const T* p = x + (live ? row : 0) * x_stride;
-    const int w = live ? width : 0, room = live ? q_room : 0;
+    const int64_t row_at = (int64_t)blockIdx.x * G + threadIdx.x / TPR;
+    const bool live = row_at < rows;
+    const int64_t row = live ? row_at : rows - 1;
+    const T* p = x + row * x_stride;
+    int8_t* out = q + row * q_stride;
     Chunk<T> v[NV ? NV : 1];
+    Columns at[NV ? NV : 1];
     float amax = 0.f;
-    auto add = [&](const Chunk<T>& c) {                                        // (values behind the row are 0)
+    auto add = [&](const Chunk<T>& c) {                                        // (values read twice, or 0 behind the row, change no maximum)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) amax = fmaxf(amax, abs_or_inf((float)c.v[j]));
     };
     if constexpr (NV > 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = load_chunk(p + (t + i * TPR) * VEC, w - (t + i * TPR) * VEC);
+        for (int i = 0; i < NV; ++i) {
+            at[i] = columns<VEC>(t + i * TPR, width);
+            v[i] = load_all<T, VEC>(p + at[i].start);
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) add(v[i]);
     } else
-        for (int c = t * VEC; c < w; c += TPR * VEC) add(load_chunk(p + c, w - c));
+        for (int c = t * VEC; c < width; c += TPR * VEC) add(load_chunk(p + c, width - c));
     amax = wave_max(amax);
     if constexpr (TPR > 64) {
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = amax;
         __syncthreads();
         amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     }
+    if (!live) return;
     const float scale = row_scale(amax);
-    if (live && t == 0) scales[row] = scale;
-    auto put = [&](const Chunk<T>& c, int c0) {
-        int8_t o[VEC], *out = q + (live ? row : 0) * q_stride + c0;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = (int8_t)quantize_value((float)c.v[j], scale);
-        if (room - c0 >= VEC) __builtin_memcpy(out, o, VEC);
-        else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) if (j < room - c0) out[j] = o[j];
-        }
+    if (t == 0) scales[row] = scale;
+    if (t < q_room - width) out[width + t] = 0;                                // the padding (less than 16 bytes)
+    const float inverse = 1.f / scale;
+    auto quantized = [&](const Chunk<T>& c) {
+        float f[VEC];
+        widen(c, 0, f);
+        return quantize_values(f, scale, inverse);
     };
     if constexpr (NV > 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) put(v[i], (t + i * TPR) * VEC);
+        for (int i = 0; i < NV; ++i) {
+            const Chunk<int8_t, VEC> o = quantized(v[i]);
+            if (at[i].first <= 0) __builtin_memcpy(out + at[i].start, &o, VEC);
+            else if (at[i].first < VEC)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) if (j >= at[i].first) out[at[i].start + j] = o.v[j];
+        }
     } else
-        for (int c = t * VEC; c < room; c += TPR * VEC) put(load_chunk(p + c, w - c), c);
+        for (int c = t * VEC; c < width; c += TPR * VEC) store_chunk(out + c, quantized(load_chunk(p + c, width - c)), width - c);
 }
 
 template <typename T, int TPR, int NV>
@@ -184,7 +274,8 @@ template <typename T>
 void quantize(const void* x, int64_t rows, int width, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, hipStream_t st) {
     const int room = (int)std::min<int64_t>(q_stride, ceil_div64(width, 16) * 16), chunks = (int)ceil_div64(width, Chunk<T>::N);
     auto go = [&](auto f) { f(x, rows, width, x_stride, q, q_stride, room, scale, st); };
-    if (chunks <= 64) go(launch_quantize<T, 64, 1>);
+    if (width < Chunk<T>::N) go(launch_quantize<T, 64, 0>);
+    else if (chunks <= 64) go(launch_quantize<T, 64, 1>);
     else if (chunks <= 128) go(launch_quantize<T, 64, 2>);
     else if (chunks <= 256) go(launch_quantize<T, 64, 4>);
     else if (chunks <= 512) go(launch_quantize<T, 256, 2>);
@@ -214,6 +305,12 @@ int check_int8(const spi_linear_int8_desc* d, const char* who) {
     return SPI_OK;
 }
 int64_t q_pitch(int K) { return ceil_div64(K, 16) * 16; }
+bool few_rows(const spi_linear_int8_desc& d) { return d.M <= FEW && d.M * few_pitch(d.K) <= FEW_LDS; }
+bool few_floats(const spi_linear_int8_desc& d) { return few_rows(d) && d.M <= FEW_FLOATS && d.x_dtype != SPI_DTYPE_I8; }
+template <typename T>
+void launch_few(const spi_linear_int8_desc& d, const Int8Args& a, const void* x, int64_t x_stride, hipStream_t st) {
+    hipLaunchKernelGGL(int8_few_rows_kernel<T>, dim3((unsigned)ceil_div64(d.N, FEW)), dim3(256), (size_t)d.M * few_pitch(d.K), st, a, (const T*)x, x_stride, d.w_bytes);
+}
 
 // ---- ragged groups -----------------------------------------------------------------------------------------------------------------------
 struct GroupArgs {
@@ -225,8 +322,8 @@ struct GroupArgs {
 };
 
 enum { PASS_FWD = 0, PASS_DGRAD = 1, PASS_WGRAD = 2 };
-template <typename T, int PASS, int SIZE, bool DMA>
-using PassEngine = Engine<T, SIZE, PASS == PASS_WGRAD, PASS != PASS_FWD, DMA>;
+template <typename T, int PASS, int SIZE, int LOAD>
+using PassEngine = Engine<T, SIZE, PASS == PASS_WGRAD, PASS != PASS_FWD, LOAD>;
 
 // the tile of engine E at rows t.row .. (at most t.end), columns c0 ..; of dw: at (r0, c0) of group t.e
 template <typename E, typename T, int PASS>
@@ -239,7 +336,8 @@ __device__ __forceinline__ void grouped_tile(const GroupArgs& a, const RowTile& 
     if constexpr (PASS == PASS_WGRAD) {
         const int rows = min(E::BM, a.N - r0);
         const int64_t len = t.end - t.row;
-        run({(const char*)a.dy + t.row * pn + r0 * ES, pn, len * pn - r0 * ES, len, rows}, {(const char*)a.x + t.row * pk + c0 * ES, pk, len * pk - c0 * ES, len, cols});
+        run({(const char*)a.dy + t.row * pn + r0 * ES, pn, len * pn - r0 * ES, len, rows, (a.T - t.row) * pn - r0 * ES},
+            {(const char*)a.x + t.row * pk + c0 * ES, pk, len * pk - c0 * ES, len, cols, (a.T - t.row) * pk - c0 * ES});
         E::each(acc, s0, s1, [&](int i, int j, f32x4_t v) {
             if (i >= rows || j >= cols) return;
             const float y[4] = {v[0] * a.gain, v[1] * a.gain, v[2] * a.gain, v[3] * a.gain};
@@ -250,9 +348,10 @@ __device__ __forceinline__ void grouped_tile(const GroupArgs& a, const RowTile& 
         if (t.e >= 0) {
             const int64_t pi = PASS == PASS_FWD ? pk : pn;
             const char* w = (const char*)a.w + (int64_t)t.e * a.N * pk;
-            const TileOperand A{(const char*)(PASS == PASS_FWD ? a.x : a.dy) + t.row * pi, pi, rows * pi, inner, rows};
-            if constexpr (PASS == PASS_FWD) run(A, {w + c0 * pk, pk, cols * pk, inner, cols});
-            else run(A, {w + c0 * ES, pk, inner * pk - c0 * ES, inner, cols});
+            const TileOperand A{(const char*)(PASS == PASS_FWD ? a.x : a.dy) + t.row * pi, pi, rows * pi, inner, rows, (a.T - t.row) * pi};
+            const int64_t end = (int64_t)(a.E - t.e) * a.N * pk;
+            if constexpr (PASS == PASS_FWD) run(A, {w + c0 * pk, pk, cols * pk, inner, cols, end - c0 * pk});
+            else run(A, {w + c0 * ES, pk, inner * pk - c0 * ES, inner, cols, end - c0 * ES});
         }
         const T* bias = PASS == PASS_FWD && a.bias && t.e >= 0 ? (const T*)a.bias + (int64_t)t.e * a.N + c0 : nullptr;
         T* out = (T*)(PASS == PASS_FWD ? a.y : a.dx) + (int64_t)t.row * width + c0;
@@ -271,9 +370,9 @@ constexpr int CUS = 256;
 __device__ __forceinline__ int whole_tiles(int tiles) { const int last = tiles % CUS; return last <= CUS / 2 ? tiles - last : tiles; }
 int64_t most_blocks(int64_t tiles) { return tiles + 3 * (CUS / 2); }
 
-template <typename T, int PASS, int SIZE, bool DMA>
+template <typename T, int PASS, int SIZE, int LOAD>
 __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) grouped_tile_kernel(const GroupArgs a) {
-    typedef PassEngine<T, PASS, SIZE, DMA> E;
+    typedef PassEngine<T, PASS, SIZE, LOAD> E;
     __shared__ __attribute__((aligned(1024))) char s0[E::STAGE], s1[E::STAGE];
     const int width = PASS == PASS_FWD ? a.N : a.K, cols = (width + SIZE - 1) / SIZE;
     const int rows = PASS == PASS_WGRAD ? (a.N + SIZE - 1) / SIZE : count_tiles(a.offsets, a.E, a.T, SIZE), tiles = rows * cols * (PASS == PASS_WGRAD ? a.E : 1);
@@ -294,7 +393,7 @@ __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) grouped_tile_kernel(c
     int c0 = col * SIZE;
     if constexpr (SIZE == 256) {
         if (cut >= 0) {
-            typedef TileEngine<T, 128, 128, 2, 4, PASS == PASS_WGRAD, PASS != PASS_FWD, DMA> Q;
+            typedef TileEngine<T, 128, 128, 2, 4, PASS == PASS_WGRAD, PASS != PASS_FWD, LOAD> Q;
             const int down = cut % 4 / 2 * 128, right = cut % 2 * 128;
             c0 += right;
             if (PASS == PASS_WGRAD) r0 += down;
@@ -306,32 +405,31 @@ __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) grouped_tile_kernel(c
     grouped_tile<E, T, PASS>(a, t, r0, c0, s0, s1);
 }
 // db[e][n] = sum of dy over the group's rows, in two steps of a fixed order: part s of S of the group's rows into part [E][S][N] (S = 1: straight into db), then the
-// parts.  A block takes 64 chunks of 16 bytes by four rows at a time.
-template <typename T>
+// parts.  A block takes 64 chunks of VEC columns by four rows at a time.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256) grouped_bias_grad_kernel(const GroupArgs a, float* __restrict__ part, int S) {
-    constexpr int N = Chunk<T>::N;
-    __shared__ float sum[4][64][N + 1];
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = (blockIdx.x * 64 + c) * N, s = blockIdx.y, e = blockIdx.z;
+    __shared__ float sum[4][64][VEC + 1];
+    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, s = blockIdx.y, e = blockIdx.z;
+    const Columns at = columns<VEC>(blockIdx.x * 64 + c, a.N);
     const RowTile t = group_rows(a.offsets, a.T, e);
     const int64_t len = t.end - t.row, from = t.row + len * s / S, to = t.row + len * (s + 1) / S;
-    float v[N] = {};
-    if (n < a.N)
-#pragma unroll 4
-        for (int64_t row = from + r; row < to; row += 4) {
-            const Chunk<T> x = load_chunk((const T*)a.dy + row * a.N + n, a.N - n);
+    float v[VEC] = {};
+    const T* p = (const T*)a.dy + at.start;
+#pragma unroll 8
+    for (int64_t row = from + r; row < to; row += 4) {
+        const Chunk<T, VEC> x = load_all<T, VEC>(p + row * a.N);
 #pragma unroll
-            for (int j = 0; j < N; ++j) v[j] += (float)x.v[j];
-        }
-#pragma unroll
-    for (int j = 0; j < N; ++j) sum[r][c][j] = v[j];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * N; i += 256) {
-        const int cc = i / N, j = i % N, col = blockIdx.x * 64 * N + i;
-        if (col >= a.N) break;
-        const float x = (sum[0][cc][j] + sum[1][cc][j]) + (sum[2][cc][j] + sum[3][cc][j]);
-        if (S > 1) part[((int64_t)e * S + s) * a.N + col] = x;
-        else ((T*)a.db)[(int64_t)e * a.N + col] = (T)x;
+        for (int j = 0; j < VEC; ++j) v[j] += (float)x.v[j];
     }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum[r][c][j] = v[j];
+    __syncthreads();
+    if (r) return;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = (sum[0][c][j] + sum[1][c][j]) + (sum[2][c][j] + sum[3][c][j]);
+    if (at.first >= VEC) return;
+    if (S > 1) store_columns(part + ((int64_t)e * S + s) * a.N + at.start, v, at.first);
+    else store_columns((T*)a.db + (int64_t)e * a.N + at.start, v, at.first);
 }
 template <typename T>
 __global__ void __launch_bounds__(256) grouped_bias_join_kernel(const GroupArgs a, const float* __restrict__ part, int S) {
@@ -339,19 +437,25 @@ __global__ void __launch_bounds__(256) grouped_bias_join_kernel(const GroupArgs 
     if (i >= (int64_t)a.E * a.N) return;
     const float* p = part + i / a.N * S * a.N + i % a.N;
     float v = 0.f;
+#pragma unroll 16
     for (int s = 0; s < S; ++s) v += p[(int64_t)s * a.N];
     ((T*)a.db)[i] = (T)v;
 }
 // parts of a group's rows: enough blocks for the chip (four for each CU), no part under 64 rows of an average group
 int bias_parts(const spi_grouped_linear_desc& d) {
     const int64_t blocks = ceil_div64(d.N, 64 * (d.dtype == SPI_DTYPE_F32 ? 4 : 8)) * d.E;
-    return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div64(1024, blocks), d.T / d.E / 64, 64}));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({ceil_div64(1024, blocks), d.T / d.E / 64, 32}));
+}
+template <typename T, int VEC>
+void bias_grad(const spi_grouped_linear_desc& d, const GroupArgs& a, hipStream_t st) {
+    const int S = bias_parts(d);
+    hipLaunchKernelGGL((grouped_bias_grad_kernel<T, VEC>), dim3((unsigned)ceil_div64(d.N, 64 * VEC), (unsigned)S, (unsigned)d.E), dim3(256), 0, st, a, (float*)d.workspace, S);
+    if (S > 1) hipLaunchKernelGGL(grouped_bias_join_kernel<T>, dim3((unsigned)ceil_div64((int64_t)d.E * d.N, 256)), dim3(256), 0, st, a, (const float*)d.workspace, S);
 }
 template <typename T>
 void bias_grad(const spi_grouped_linear_desc& d, const GroupArgs& a, hipStream_t st) {
-    const int S = bias_parts(d);
-    hipLaunchKernelGGL(grouped_bias_grad_kernel<T>, dim3((unsigned)ceil_div64(d.N, 64 * Chunk<T>::N), (unsigned)S, (unsigned)d.E), dim3(256), 0, st, a, (float*)d.workspace, S);
-    if (S > 1) hipLaunchKernelGGL(grouped_bias_join_kernel<T>, dim3((unsigned)ceil_div64((int64_t)d.E * d.N, 256)), dim3(256), 0, st, a, (const float*)d.workspace, S);
+    if (d.N >= Chunk<T>::N) bias_grad<T, Chunk<T>::N>(d, a, st);
+    else bias_grad<T, 1>(d, a, st);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -364,10 +468,10 @@ int tile_edge(F rows, int64_t width, bool dma) {
     if (dma && rows(256) * ceil_div64(width, 256) >= CUS) return 256;
     return rows(128) * ceil_div64(width, 128) >= (dma ? CUS : CUS * 3 / 2) ? 128 : 64;
 }
-template <typename T, int PASS, int SIZE, bool DMA>
+template <typename T, int PASS, int SIZE, int LOAD>
 void launch_tiles(const GroupArgs& a, hipStream_t st) {
     const int64_t tiles = PASS == PASS_WGRAD ? ceil_div64(a.N, SIZE) * ceil_div64(a.K, SIZE) * a.E : most_tiles(a.T, a.E, SIZE) * ceil_div64(PASS == PASS_FWD ? a.N : a.K, SIZE);
-    hipLaunchKernelGGL((grouped_tile_kernel<T, PASS, SIZE, DMA>), dim3((unsigned)(SIZE == 256 ? most_blocks(tiles) : tiles)), dim3(SIZE == 256 ? 512 : 256), 0, st, a);
+    hipLaunchKernelGGL((grouped_tile_kernel<T, PASS, SIZE, LOAD>), dim3((unsigned)(SIZE == 256 ? most_blocks(tiles) : tiles)), dim3(SIZE == 256 ? 512 : 256), 0, st, a);
 }
 template <typename T, int PASS>
 void grouped_pass(const GroupArgs& a, hipStream_t st) {
@@ -376,11 +480,13 @@ void grouped_pass(const GroupArgs& a, hipStream_t st) {
     const int64_t width = PASS == PASS_FWD ? a.N : a.K;
     auto rows = [&](int size) { return PASS == PASS_WGRAD ? ceil_div64(a.N, size) * a.E : a.T / size + std::min(a.T, a.E) / 2; };        // (of ragged groups half a tile each is empty)
     const int size = tile_edge(rows, width, dma);
-    if (size == 256) launch_tiles<T, PASS, 256, true>(a, st);
-    else if (size == 128 && dma) launch_tiles<T, PASS, 128, true>(a, st);
-    else if (size == 128) launch_tiles<T, PASS, 128, false>(a, st);
-    else if (dma) launch_tiles<T, PASS, 64, true>(a, st);
-    else launch_tiles<T, PASS, 64, false>(a, st);
+    const int64_t smallest = std::min({(int64_t)a.T * a.K, (int64_t)a.T * a.N, (int64_t)a.E * a.N * a.K}) * ES;
+    if (size == 256) launch_tiles<T, PASS, 256, LOAD_DMA>(a, st);
+    else if (size == 128 && dma) launch_tiles<T, PASS, 128, LOAD_DMA>(a, st);
+    else if (size == 128) launch_tiles<T, PASS, 128, LOAD_WIDE>(a, st);
+    else if (dma) launch_tiles<T, PASS, 64, LOAD_DMA>(a, st);
+    else if (smallest >= 16) launch_tiles<T, PASS, 64, LOAD_WIDE>(a, st);
+    else launch_tiles<T, PASS, 64, LOAD_EACH>(a, st);
 }
 template <int PASS>
 void grouped_pass(int dtype, const GroupArgs& a, hipStream_t st) {
@@ -417,7 +523,7 @@ extern "C" int spi_quantize_rows(const void* x, int64_t rows, int width, int64_t
 
 extern "C" int spi_sizeof_linear_int8_desc(void) { return (int)sizeof(spi_linear_int8_desc); }
 extern "C" int64_t spi_linear_int8_workspace(const spi_linear_int8_desc* d) {
-    if (check_int8(d, "spi_linear_int8_workspace") || d->x_dtype == SPI_DTYPE_I8) return 0;
+    if (check_int8(d, "spi_linear_int8_workspace") || d->x_dtype == SPI_DTYPE_I8 || few_floats(*d)) return 0;
     return d->M * (q_pitch(d->K) + (int64_t)sizeof(float));
 }
 extern "C" int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t stream) {
@@ -426,6 +532,13 @@ extern "C" int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t strea
     SPI_REQUIRE(d->workspace_bytes >= spi_linear_int8_workspace(d) && (d->workspace || d->workspace_bytes == 0), "spi_linear_int8: workspace too small");
     hipStream_t st = as_stream(stream);
     Int8Args a{(const int8_t*)d->x, d->x_scale, d->w, d->w_scale, d->bias, d->y, d->x_stride, d->w_stride, (int)d->M, d->N, d->K, d->y_dtype, d->act, d->alpha, d->gain, d->clamp};
+    if (few_floats(*d)) {
+        if (d->x_dtype == SPI_DTYPE_F32) launch_few<float>(*d, a, d->x, d->x_stride, st);
+        else if (d->x_dtype == SPI_DTYPE_F16) launch_few<half_t>(*d, a, d->x, d->x_stride, st);
+        else launch_few<bf16_t>(*d, a, d->x, d->x_stride, st);
+        SPI_LAUNCH_CHECK("spi_linear_int8");
+        return SPI_OK;
+    }
     if (d->x_dtype != SPI_DTYPE_I8) {
         a.q = (int8_t*)d->workspace;
         a.q_stride = q_pitch(d->K);
@@ -433,16 +546,22 @@ extern "C" int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t strea
         quantize_any(d->x, d->M, d->K, d->x_stride, d->x_dtype, (int8_t*)a.q, a.q_stride, (float*)a.q_scale, st);
         SPI_LAUNCH_CHECK("spi_linear_int8 (quantize)");
     }
+    if (few_rows(*d)) {
+        launch_few<int8_t>(*d, a, a.q, a.q_stride, st);
+        SPI_LAUNCH_CHECK("spi_linear_int8");
+        return SPI_OK;
+    }
     // 16-byte rows; where they do not end on 16 bytes, the rows' own padding has to be 0 and the weights' readable
     const bool dma = aligned16(a.q) && aligned16(a.w) && a.q_stride % 16 == 0 && a.w_stride % 16 == 0 &&
                      (d->K % 16 == 0 || (d->x_dtype != SPI_DTYPE_I8 && d->w_bytes >= (int64_t)(d->N - 1) * d->w_stride + q_pitch(d->K)));
     const int size = tile_edge([&](int edge) { return ceil_div64(d->M, edge); }, d->N, dma), rows = (int)ceil_div64(d->M, size), cols = (int)ceil_div64(d->N, size);
     const dim3 grid((unsigned)rows * (unsigned)cols);
-    if (size == 256) hipLaunchKernelGGL((int8_tile_kernel<256, true>), grid, dim3(512), 0, st, a, rows, cols);
-    else if (size == 128 && dma) hipLaunchKernelGGL((int8_tile_kernel<128, true>), grid, dim3(256), 0, st, a, rows, cols);
-    else if (size == 128) hipLaunchKernelGGL((int8_tile_kernel<128, false>), grid, dim3(256), 0, st, a, rows, cols);
-    else if (dma) hipLaunchKernelGGL((int8_tile_kernel<64, true>), grid, dim3(256), 0, st, a, rows, cols);
-    else hipLaunchKernelGGL((int8_tile_kernel<64, false>), grid, dim3(256), 0, st, a, rows, cols);
+    if (size == 256) hipLaunchKernelGGL((int8_tile_kernel<256, LOAD_DMA>), grid, dim3(512), 0, st, a, rows, cols);
+    else if (size == 128 && dma) hipLaunchKernelGGL((int8_tile_kernel<128, LOAD_DMA>), grid, dim3(256), 0, st, a, rows, cols);
+    else if (size == 128) hipLaunchKernelGGL((int8_tile_kernel<128, LOAD_WIDE>), grid, dim3(256), 0, st, a, rows, cols);
+    else if (dma) hipLaunchKernelGGL((int8_tile_kernel<64, LOAD_DMA>), grid, dim3(256), 0, st, a, rows, cols);
+    else if ((d->M - 1) * a.q_stride + d->K >= 16 && (d->N - 1) * a.w_stride + d->K >= 16) hipLaunchKernelGGL((int8_tile_kernel<64, LOAD_WIDE>), grid, dim3(256), 0, st, a, rows, cols);
+    else hipLaunchKernelGGL((int8_tile_kernel<64, LOAD_EACH>), grid, dim3(256), 0, st, a, rows, cols);
     SPI_LAUNCH_CHECK("spi_linear_int8");
     return SPI_OK;
 }

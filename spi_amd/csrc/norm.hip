@@ -165,15 +165,14 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(const N
         }
         if (d.q) {
             const float scale = row_scale(row_max<TPR>(amax, red, phase));
+            const float inverse = 1.f / scale;
             int8_t* q = d.q + row * d.q_stride;
             if (live) {
                 if (t == 0) d.q_scale[row] = scale;
                 if (t < d.q_stride - d.width) q[d.width + t] = 0;              // the padding (less than 16 bytes)
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
-                    Chunk<int8_t, VEC> v;
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) v.v[j] = (int8_t)quantize_value(s[i][j], scale);
+                    const Chunk<int8_t, VEC> v = quantize_values(s[i], scale, inverse);
                     if (first[i] <= 0) __builtin_memcpy(q + at[i], &v, VEC);
                     else if (first[i] < VEC)
 #pragma unroll

@@ -45,24 +45,30 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 // One operand of a tile.  p: its first value; pitch: bytes between neighbours on the axis that is not adjacent; k: values of the summed axis; n: valid values of the
 // tile's own axis; bytes: what may be read from p on (row: n * pitch; col: k * pitch less the bytes of a row before p).  256 * pitch < 2^31.
 // Summed values behind k are 0 in the tile; so are rows behind n of a `row` operand.  Columns behind n of a `col` operand may hold what follows in memory: they only reach
-// results that lie outside, too.
-struct TileOperand { const char* p; int64_t pitch, bytes, k; int n; };
+// results that lie outside, too.  end: bytes from p to the end of the tensor that the operand is part of.
+struct TileOperand { const char* p; int64_t pitch, bytes, k; int n; int64_t end; };
 
 // row: which chunk a tile row's chunks are XORed with, so that 16 rows' chunks c fall on all of the 64 banks (and eight rows' on 32)
 __device__ __forceinline__ int row_swizzle(int r) { return (r & 7) ^ ((r >> 3) & 1); }
 
-// DMA: memory -> LDS without registers, for operands whose rows begin on 16 bytes and (row) hold a whole number of 16-byte chunks; reads outside are answered with 0 by the
-// buffer's bounds check.  Otherwise through registers (`fetch` before a step's products, `put` behind them), with 16-byte loads at any alignment and the rows' last
-// values one by one.
-template <typename T, int R, int NW, bool COL, bool DMA>
+// How a stage is filled.
+//   LOAD_DMA   memory -> LDS without registers: rows that begin on 16 bytes and (row) hold a whole number of 16-byte chunks; reads outside are answered with 0 by the buffer's
+//              bounds check
+//   LOAD_WIDE  through registers (`fetch` before a step's products, `put` behind them), 16 bytes at a time at any alignment, without a condition -- a load under a condition
+//              would be waited for at once.  A chunk that would pass the tensor's end is read from its last 16 bytes and moved into place by `put`, which also clears what lies
+//              behind the summed axis
+//   LOAD_EACH  value by value where a tensor has less than 16 bytes
+enum { LOAD_DMA, LOAD_WIDE, LOAD_EACH };
+template <typename T, int R, int NW, bool COL, int LOAD>
 struct TileLoader {
     static constexpr int ES = (int)sizeof(T), KT = 128 / ES, PER = R / 8 / NW, ROW = COL ? R * ES : 128, RPI = 1024 / ROW, CHUNKS = ROW / 16;
     static_assert(R % (8 * NW) == 0 && NW % 2 == 0 && ROW <= 1024, "a wave copies 1024 bytes at a time");
     const char* base;
-    int64_t pitch, left, k;                   // left: bytes from `base` to the operand's end; k: values of the summed axis still to come
+    int64_t pitch, left, k;                   // left: bytes from `base` to the operand's (LOAD_WIDE: the tensor's) end; k: values of the summed axis still to come
     int n;
     unsigned voff[PER];
-    i32x4_t hold[DMA ? 1 : PER];
+    i32x4_t hold[LOAD == LOAD_DMA ? 1 : PER];
+    int moved[LOAD == LOAD_WIDE ? PER : 1];   // bytes by which a held chunk was read too early
 
     // col: where the chunks of summed row kr lie; keeps the 8 rows x 64 bytes of a transposing read (16-bit) and the two 128-byte halves of a float read apart
     static __device__ __forceinline__ int swizzle(int kr) {
@@ -76,7 +82,7 @@ struct TileLoader {
         c = (lane % CHUNKS) ^ (COL ? swizzle(r) : row_swizzle(r));
     }
     __device__ __forceinline__ void init(const TileOperand& o) {
-        base = o.p; pitch = o.pitch; k = o.k; n = o.n; left = o.bytes;
+        base = o.p; pitch = o.pitch; k = o.k; n = o.n; left = LOAD == LOAD_WIDE ? o.end : o.bytes;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             int r, c;
@@ -86,7 +92,7 @@ struct TileLoader {
     }
     // starts the copies of the next step (DMA: into `stage`, R * 128 bytes)
     __device__ __forceinline__ void fetch(char* stage) {
-        if constexpr (DMA) {
+        if constexpr (LOAD == LOAD_DMA) {
             const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
             const int64_t most = (int64_t)(COL ? KT : R) * pitch;
             const __amdgpu_buffer_rsrc_t rs = make_rsrc(base, left > 0 ? (left < most ? left : most) : 0);
@@ -96,6 +102,14 @@ struct TileLoader {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(stage + (wave + i * NW) * 1024), 16, whole ? voff[i] : BUF_OOB, 0, 0, 0);
+        } else if constexpr (LOAD == LOAD_WIDE) {
+            const int last = (int)max(min(left - 16, (int64_t)0x7fffffff), -(int64_t)0x7fffffff);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int at = min((int)voff[i], last);
+                moved[i] = (int)voff[i] - at;
+                hold[i] = __builtin_bit_cast(i32x4_t, load_all<char, 16>(base + at));
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
@@ -110,10 +124,24 @@ struct TileLoader {
         left -= step;
         k -= KT;
     }
-    __device__ __forceinline__ void put(char* stage) const {
-        if constexpr (!DMA)
+    __device__ __forceinline__ void put(char* stage) {
+        if constexpr (LOAD != LOAD_DMA)
 #pragma unroll
-            for (int i = 0; i < PER; ++i) *reinterpret_cast<i32x4_t*>(stage + ((threadIdx.x >> 6) + i * NW) * 1024 + (threadIdx.x & 63) * 16) = hold[i];
+            for (int i = 0; i < PER; ++i) {
+                if constexpr (LOAD == LOAD_WIDE) {
+                    int r, c;
+                    place(i, r, c);
+                    const int64_t before = k + KT, valid = COL ? (r < before ? 16 : 0) : (before - c * (16 / ES)) * ES;      // bytes of the chunk on the summed axis
+                    if (moved[i] | (valid < 16)) {
+                        typedef unsigned __int128 u128;
+                        u128 v = __builtin_bit_cast(u128, hold[i]);
+                        v = moved[i] < 16 ? v >> (moved[i] * 8) : (u128)0;
+                        if (valid < 16) v &= valid > 0 ? ((u128)1 << (int)(valid * 8)) - 1 : (u128)0;
+                        hold[i] = __builtin_bit_cast(i32x4_t, v);
+                    }
+                }
+                *reinterpret_cast<i32x4_t*>(stage + ((threadIdx.x >> 6) + i * NW) * 1024 + (threadIdx.x & 63) * 16) = hold[i];
+            }
     }
 };
 
@@ -161,7 +189,7 @@ struct TileReader {
 
 // Two stages of LDS: the copies of step k + 1 are under way while step k is multiplied, one barrier a step.  (Four stages, and steps of 64 bytes, were measured slower:
 // 16384 x 2048 x 2048 bf16 at 256 x 256, 143 us against 132: half cache lines, and the latency is already covered.)
-template <typename T, int BM_, int BN_, int GM_, int GN_, bool COLA, bool COLB, bool DMA>
+template <typename T, int BM_, int BN_, int GM_, int GN_, bool COLA, bool COLB, int LOAD>
 struct TileEngine {
     static constexpr int BM = BM_, BN = BN_, GM = GM_, GN = GN_, NW = GM * GN, WM = BM / GM, WN = BN / GN, FM = WM / 32, FN = WN / 32, KT = 128 / (int)sizeof(T),
                          STAGE = (BM + BN) * 128;
@@ -171,8 +199,8 @@ struct TileEngine {
     // s0, s1: LDS arrays of their own (the compiler then knows that the copies into one do not touch the reads of the other)
     static __device__ __forceinline__ void run(const TileOperand& a, const TileOperand& b, char* s0, char* s1, Accs& acc) {
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        TileLoader<T, BM, NW, COLA, DMA> la;
-        TileLoader<T, BN, NW, COLB, DMA> lb;
+        TileLoader<T, BM, NW, COLA, LOAD> la;
+        TileLoader<T, BN, NW, COLB, LOAD> lb;
         TileReader<T, BM, COLA, FM> ra;
         TileReader<T, BN, COLB, FN> rb;
         la.init(a);
@@ -195,6 +223,7 @@ struct TileEngine {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
                 if (kk < 3) read(kk + 1);
+                __builtin_amdgcn_sched_barrier(0);               // (the compiler would put these reads behind the products, and then wait for them)
 #pragma unroll
                 for (int q = 0; q < Mma<T>::N; ++q)              // (the steps of one accumulator apart: each waits for the one before it)
 #pragma unroll

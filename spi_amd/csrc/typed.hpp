@@ -126,4 +126,28 @@ __device__ __forceinline__ int quantize_value(float v, float scale) {          /
     const float q = scale > 0.f ? rintf(v / scale) : 0.f;
     return (int)fminf(fmaxf(q, -127.f), 127.f);
 }
+// N values of a row by its scale.  The IEEE quotient only where it could round to another integer than the product with 1 / scale does: the two are within
+// 127 * (2^-23 + 2^-24) < 2.3e-5 of each other.  (8192 x 4096 bf16 with a division for each value: 29 us, of which 20 are memory's.)
+template <int N>
+__device__ __forceinline__ Chunk<int8_t, N> quantize_values(const float (&v)[N], float scale, float inverse) {
+    Chunk<int8_t, N> q;
+    if (!(scale >= 0x1p-100f)) {                                               // zeros, NaN, and scales whose inverse is far from exact
+#pragma unroll
+        for (int j = 0; j < N; ++j) q.v[j] = (int8_t)quantize_value(v[j], scale);
+        return q;
+    }
+    float r[N], off = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float x = v[j] * inverse;
+        r[j] = rintf(x);
+        off = fmaxf(off, fabsf(x - r[j]));
+    }
+    if (off > 0.5f - 1e-4f)
+#pragma unroll
+        for (int j = 0; j < N; ++j) r[j] = rintf(v[j] / scale);
+#pragma unroll
+    for (int j = 0; j < N; ++j) q.v[j] = (int8_t)(int)r[j];
+    return q;
+}
 #endif

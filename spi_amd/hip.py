@@ -4,7 +4,6 @@ Thin by design: tensors go down as raw device pointers + sizes + the current HIP
 are allocated by the caller with ``torch.empty``.  There is NO fallback: if the library cannot be
 loaded, or a tensor is not a contiguous fp32 GPU tensor, the call raises.
 """
-import contextlib
 import ctypes
 import os
 import torch
@@ -196,9 +195,12 @@ def same_device(*tensors):
     return device
 
 
-def on(device):
-    """Context in which `device` is the current one: launches go to ITS current stream, workspaces come from its memory."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def on(device, fn, *args):
+    """fn(*args) with `device` as the current one: launches go to ITS current stream, workspaces come from its memory."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
 
 
 def ptr_any(t):

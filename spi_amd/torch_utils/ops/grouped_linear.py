@@ -17,11 +17,12 @@ def _desc(cfg, x, weight, offsets):
 
 
 def _launch(name, pass_id, d, device):
-    nbytes = hip.lib().spi_grouped_linear_workspace(ctypes.byref(d), pass_id)
+    ref = ctypes.byref(d)
+    nbytes = hip.lib().spi_grouped_linear_workspace(ref, pass_id)
     if nbytes:
         workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
         d.workspace, d.workspace_bytes = workspace.data_ptr(), nbytes
-    hip.call(name, ctypes.byref(d), hip.stream())
+    hip.call(name, ref, hip.stream())
 
 
 def _forward(cfg, x, weight, bias, offsets):
@@ -43,25 +44,29 @@ class _GroupedLinear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, offsets = ctx.saved_tensors
-        dx = dw = db = None
-        with hip.on(x.device):
-            dy = dy.contiguous()
-            if ctx.needs_input_grad[1]:
-                dx = torch.empty_like(x)
-                d = _desc(ctx.cfg, None, weight, offsets)
-                d.dy, d.dx = dy.data_ptr(), dx.data_ptr()
-                _launch('spi_grouped_linear_dgrad', 1, d, x.device)
-            if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
-                d = _desc(ctx.cfg, x, None, offsets)
-                d.dy = dy.data_ptr()
-                if ctx.needs_input_grad[2]:
-                    dw = torch.empty_like(weight)
-                    d.dw = dw.data_ptr()
-                if ctx.needs_input_grad[3]:
-                    db = torch.empty(weight.shape[:2], device=x.device, dtype=x.dtype)
-                    d.db = db.data_ptr()
-                _launch('spi_grouped_linear_wgrad', 2, d, x.device)
-        return None, dx, dw, db, None
+        return (None, *hip.on(x.device, _backward, ctx.cfg, ctx.needs_input_grad[1:4], x, weight, offsets, dy), None)
+
+
+def _backward(cfg, need, x, weight, offsets, dy):
+    dx = dw = db = None
+    if not dy.is_contiguous():
+        dy = dy.contiguous()
+    if need[0]:
+        dx = torch.empty_like(x)
+        d = _desc(cfg, None, weight, offsets)
+        d.dy, d.dx = dy.data_ptr(), dx.data_ptr()
+        _launch('spi_grouped_linear_dgrad', 1, d, x.device)
+    if need[1] or need[2]:
+        d = _desc(cfg, x, None, offsets)
+        d.dy = dy.data_ptr()
+        if need[1]:
+            dw = torch.empty_like(weight)
+            d.dw = dw.data_ptr()
+        if need[2]:
+            db = torch.empty(weight.shape[:2], device=x.device, dtype=x.dtype)
+            d.db = db.data_ptr()
+        _launch('spi_grouped_linear_wgrad', 2, d, x.device)
+    return dx, dw, db
 
 
 def grouped_linear(x, weight, offsets, bias=None, gain=1.0):
@@ -81,7 +86,6 @@ def grouped_linear(x, weight, offsets, bias=None, gain=1.0):
     x, weight, offsets = x.contiguous(), weight.contiguous(), offsets.contiguous()
     bias = None if bias is None else bias.contiguous()
     cfg = (x.shape[0], weight.shape[0], weight.shape[1], x.shape[1], hip.ROW_DTYPES[x.dtype], float(gain))
-    with hip.on(device):
-        if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-            return _GroupedLinear.apply(cfg, x, weight, bias, offsets)
-        return _forward(cfg, x, weight, bias, offsets)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return hip.on(device, _GroupedLinear.apply, cfg, x, weight, bias, offsets)
+    return hip.on(device, _forward, cfg, x, weight, bias, offsets)

@@ -15,6 +15,8 @@ MAX_IN_FEATURES = 131071         # SPI_LINEAR_INT8_MAX_K: 127 * 127 * in_feature
 
 def _rows(x):
     """[..., K] -> [rows, K] with adjacent values, and rows that are K .. 2^22 values apart"""
+    if x.ndim == 2 and x.is_contiguous():
+        return x
     k = x.shape[-1]
     x = x.reshape(-1, k)
     return x if (k == 1 or x.stride(1) == 1) and (x.shape[0] <= 1 or k <= x.stride(0) <= 1 << 22) else x.contiguous()
@@ -32,14 +34,16 @@ def quantize_rows(x):
         raise ValueError(f'rows of {tuple(x.shape)[-1:]} values: 1 to {MAX_IN_FEATURES}')
     if x.dtype not in hip.ROW_DTYPES:
         raise TypeError(f'rows of {x.dtype}: float32, float16 or bfloat16')
-    device = hip.same_device(x)
+    return hip.on(hip.same_device(x), _quantize, x)
+
+
+def _quantize(x):
     k = x.shape[-1]
     pitch = (k + 15) // 16 * 16
-    with hip.on(device):
-        q = torch.empty(x.shape[:-1] + (pitch,), device=device, dtype=torch.int8)
-        scale = torch.empty(x.shape[:-1], device=device, dtype=torch.float32)
-        r = _rows(x.detach())
-        hip.call('spi_quantize_rows', r.data_ptr(), r.shape[0], k, _stride(r), hip.ROW_DTYPES[x.dtype], q.data_ptr(), pitch, scale.data_ptr(), hip.stream())
+    q = torch.empty(x.shape[:-1] + (pitch,), device=x.device, dtype=torch.int8)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    r = _rows(x.detach())
+    hip.call('spi_quantize_rows', r.data_ptr(), r.shape[0], k, _stride(r), hip.ROW_DTYPES[x.dtype], q.data_ptr(), pitch, scale.data_ptr(), hip.stream())
     return (q if pitch == k else q[..., :k]), scale
 
 
@@ -77,25 +81,32 @@ def linear_int8(x, weight_q, weight_scale, bias=None, x_scale=None, act='linear'
     out_dtype = out_dtype or (torch.float32 if int_rows else x.dtype)
     if out_dtype not in hip.ROW_DTYPES:
         raise TypeError(f'out_dtype {out_dtype}: float32, float16 or bfloat16')
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight_scale, bias, x_scale)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad) or (int_rows and x_scale.requires_grad)):
         raise RuntimeError('linear_int8: rounded rows have no gradient; call it under torch.no_grad() or on tensors that need none')
-    device = hip.same_device(x, weight_q, weight_scale, bias, x_scale)
-    with hip.on(device):
-        y = torch.empty(x.shape[:-1] + (n,), device=device, dtype=out_dtype)
-        r, w = _rows(x), _rows(weight_q)
-        m = r.shape[0]
-        if m == 0:
-            return y
+    return hip.on(hip.same_device(x, weight_q, weight_scale, bias, x_scale), _linear, x, weight_q, weight_scale, bias, x_scale, act_id, float(d_alpha if alpha is None else alpha),
+                  float(d_gain if gain is None else gain), float(-1 if clamp is None else clamp), out_dtype)
+
+
+def _linear(x, weight_q, weight_scale, bias, x_scale, act_id, alpha, gain, clamp, out_dtype):
+    n, k = weight_q.shape
+    y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=out_dtype)
+    r, w = _rows(x), _rows(weight_q)
+    m = r.shape[0]
+    if m == 0:
+        return y
+    if not weight_scale.is_contiguous():
         weight_scale = weight_scale.contiguous()
-        bias = None if bias is None else bias.contiguous()
-        x_scale = None if x_scale is None else x_scale.contiguous()
-        d = hip.LinearInt8Desc(m, n, k, hip.DTYPE_I8 if int_rows else hip.ROW_DTYPES[x.dtype], hip.ROW_DTYPES[out_dtype], _stride(r), _stride(w),
-                               w.untyped_storage().nbytes() - w.storage_offset(), r.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w.data_ptr(),
-                               weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), act_id, float(d_alpha if alpha is None else alpha),
-                               float(d_gain if gain is None else gain), float(-1 if clamp is None else clamp))
-        nbytes = hip.lib().spi_linear_int8_workspace(ctypes.byref(d))
-        if nbytes:
-            workspace = torch.empty(nbytes, device=device, dtype=torch.uint8)
-            d.workspace, d.workspace_bytes = workspace.data_ptr(), nbytes
-        hip.call('spi_linear_int8', ctypes.byref(d), hip.stream())
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    if x_scale is not None and not x_scale.is_contiguous():
+        x_scale = x_scale.contiguous()
+    d = hip.LinearInt8Desc(m, n, k, hip.DTYPE_I8 if x_scale is not None else hip.ROW_DTYPES[x.dtype], hip.ROW_DTYPES[out_dtype], _stride(r), _stride(w),
+                           w.untyped_storage().nbytes() - w.storage_offset(), r.data_ptr(), None if x_scale is None else x_scale.data_ptr(), w.data_ptr(),
+                           weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(), act_id, alpha, gain, clamp)
+    ref = ctypes.byref(d)
+    nbytes = hip.lib().spi_linear_int8_workspace(ref)
+    if nbytes:
+        workspace = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
+        d.workspace, d.workspace_bytes = workspace.data_ptr(), nbytes
+    hip.call('spi_linear_int8', ref, hip.stream())
     return y

@@ -28,7 +28,7 @@ def _p(t):
 def _desc(cfg, h, residual, gate, weights):
     """``weights``: (post_weight, post_bias, pre_weight, pre_bias).  Contiguous tensors."""
     rows, width, per_sample, mode, act, layer, after, before, scale, eps = cfg
-    w = next((t for t in weights if t is not None), None)
+    w = weights[0] if after else weights[2]
     return hip.NormResidualDesc(rows, per_sample, width, hip.ROW_DTYPES[h.dtype], 0 if w is None else hip.ROW_DTYPES[w.dtype],
                                 0 if gate is None else hip.ROW_DTYPES[gate.dtype], mode, act, layer, after, before, scale, eps, h.data_ptr(), residual.data_ptr(),
                                 _p(gate), *map(_p, weights))
@@ -74,25 +74,33 @@ class _NormResidual(torch.autograd.Function):
         if d_stream is None and d_normed is None:
             return (None,) * 8
         if d_normed is None:                             # (only the stream was used: its norm has no part in the gradients)
-            cfg = cfg[:7] + (0,) + cfg[8:]
+            cfg = cfg[:7] + (False,) + cfg[8:]
             weights = weights[:2] + [None, None]
             need = need[:5] + (False, False)
         inputs = (h, residual, gate, *weights)
-        with hip.on(h.device):
-            if cfg[0] == 0:
-                return (None, *(torch.zeros_like(t) if n else None for t, n in zip(inputs, need)))
-            grads = [torch.empty_like(t) if n else None for t, n in zip(inputs, need)]
-            d = _desc(cfg, h, residual, gate, weights)
-            d.stats = stats.data_ptr()
-            d_stream = None if d_stream is None else d_stream.contiguous()
-            d_normed = None if d_normed is None else d_normed.contiguous()
-            d.d_stream, d.d_normed = _p(d_stream), _p(d_normed)
-            d.d_h, d.d_residual, d.d_gate, d.d_post_weight, d.d_post_bias, d.d_pre_weight, d.d_pre_bias = map(_p, grads)
-            nbytes = hip.lib().spi_norm_residual_bwd_workspace(ctypes.byref(d))
-            workspace = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
-            d.workspace, d.workspace_bytes = workspace.data_ptr(), nbytes
-            hip.call('spi_norm_residual_bwd', ctypes.byref(d), hip.stream())
-        return (None, *grads)
+        return (None, *hip.on(h.device, _backward, cfg, need, stats, inputs, d_stream, d_normed))
+
+
+def _backward(cfg, need, stats, inputs, d_stream, d_normed):
+    if cfg[0] == 0:
+        return [torch.zeros_like(t) if n else None for t, n in zip(inputs, need)]
+    h, residual, gate, *weights = inputs
+    grads = [torch.empty_like(t) if n else None for t, n in zip(inputs, need)]
+    d = _desc(cfg, h, residual, gate, weights)
+    d.stats = stats.data_ptr()
+    if d_stream is not None:
+        d_stream = d_stream.contiguous()
+        d.d_stream = d_stream.data_ptr()
+    if d_normed is not None:
+        d_normed = d_normed.contiguous()
+        d.d_normed = d_normed.data_ptr()
+    d.d_h, d.d_residual, d.d_gate, d.d_post_weight, d.d_post_bias, d.d_pre_weight, d.d_pre_bias = map(_p, grads)
+    ref = ctypes.byref(d)
+    nbytes = hip.lib().spi_norm_residual_bwd_workspace(ref)
+    workspace = torch.empty(nbytes, device=h.device, dtype=torch.uint8)
+    d.workspace, d.workspace_bytes = workspace.data_ptr(), nbytes
+    hip.call('spi_norm_residual_bwd', ref, hip.stream())
+    return grads
 
 
 def _gate_mode(h, gate):
@@ -142,25 +150,31 @@ def norm_residual(h, residual, gate=None, scale=1.0, post_weight=None, post_bias
     if quantize and not before:
         raise ValueError("quantize: where='after' has no normed rows")
     weights = (post_weight, post_bias, pre_weight, pre_bias)
-    kinds = set()
+    kind = (post_weight if after else pre_weight).dtype
+    if kind is not h.dtype and kind is not torch.float32:
+        raise TypeError(f'norm weights of {kind}: float32 or {h.dtype}')
+    if gate is not None and gate.dtype is not h.dtype and gate.dtype is not torch.float32:
+        raise TypeError(f'gate of {gate.dtype}: float32 or {h.dtype}')
     for t in weights:
         if t is not None:
             if t.shape != (width,):
                 raise ValueError(f'a norm weight of {tuple(t.shape)} for rows of {width}')
-            kinds.add(t.dtype)
-    if len(kinds) > 1 or not kinds <= {torch.float32, h.dtype} or (gate is not None and gate.dtype not in (torch.float32, h.dtype)):
-        raise TypeError(f'weights {kinds} and gate {None if gate is None else gate.dtype}: float32 or {h.dtype}, all weights alike')
+            if t.dtype is not kind:
+                raise TypeError(f'norm weights of {kind} and {t.dtype}: one type for all')
     mode, per_sample = _gate_mode(h, gate)
-    inputs = (h, residual, gate) + weights
-    device = hip.same_device(*inputs)
-    wants_grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs)
+    device = hip.same_device(h, residual, gate, *weights)
+    wants_grad = False
+    if torch.is_grad_enabled():
+        for t in (h, residual, gate) + weights:
+            if t is not None and t.requires_grad:
+                wants_grad = True
+                break
     if wants_grad and quantize:
         raise RuntimeError('norm_residual: rounded rows have no gradient; call quantize=True under torch.no_grad() or on tensors that need none')
     if wants_grad and width > MAX_WIDTH_BACKWARD:
         raise ValueError(f'rows of {width} values: gradients are provided up to {MAX_WIDTH_BACKWARD}')
-    h, residual, gate, *weights = (t if t is None or t.is_contiguous() else t.contiguous() for t in inputs)
-    cfg = (h.numel() // width, width, per_sample, mode, _ba.activation_funcs[gate_act][0], int(norm == 'layer'), int(after), int(before), float(scale), float(eps))
-    with hip.on(device):
-        if wants_grad:
-            return _NormResidual.apply(cfg, h, residual, gate, *weights)
-        return _forward(cfg, h, residual, gate, weights, False, quantize)[:2]
+    h, residual, gate, *weights = [t if t is None or t.is_contiguous() else t.contiguous() for t in (h, residual, gate) + weights]
+    cfg = (h.numel() // width, width, per_sample, mode, _ba.activation_funcs[gate_act][0], norm == 'layer', after, before, float(scale), float(eps))
+    if wants_grad:
+        return hip.on(device, _NormResidual.apply, cfg, h, residual, gate, *weights)
+    return hip.on(device, _forward, cfg, h, residual, gate, weights, False, quantize)[:2]

@@ -309,7 +309,7 @@ def int8_reference(q, scale, wq, ws, bias, act, gain, clamp):
     return y, mag
 
 
-@pytest.mark.parametrize('m,n,k', [(1, 512, 512), (1, 1, 1), (2, 33, 17), (14, 512, 2048), (16, 100, 64), (17, 4096, 512), (64, 65, 300), (65, 64, 4100), (100, 333, 1003),
+@pytest.mark.parametrize('m,n,k', [(1, 512, 512), (1, 1, 1), (2, 33, 17), (14, 512, 2048), (16, 100, 64), (4, 40, 4001), (3, 4099, 33), (17, 4096, 512), (64, 65, 300), (65, 64, 4100), (100, 333, 1003),
                                    (257, 512, 129), (600, 512, 512), (1111, 770, 1031)])
 def test_linear_int8_sizes(m, n, k):
     from spi_amd.torch_utils.ops.linear_int8 import linear_int8
@@ -358,7 +358,7 @@ def test_linear_int8_exact_sums():
 
 
 def test_linear_int8_rows_stand_alone_and_strides():
-    from spi_amd.torch_utils.ops.linear_int8 import linear_int8
+    from spi_amd.torch_utils.ops.linear_int8 import linear_int8, quantize_rows
     g = gen(6)
     for m in (5, 70, 300):
         x = randn(g, m, 96)
@@ -378,6 +378,12 @@ def test_linear_int8_rows_stand_alone_and_strides():
         padded[:, :90] = wq[:, :90]                                                              # aligned rows whose padding is not zero
         assert torch.equal(linear_int8(x[:, :90], padded[:, :90], ws), linear_int8(x[:, :90], wq[:, :90].contiguous(), ws))
         assert torch.equal(linear_int8(x[:1].expand(4, 96), wq, ws), want[:1].expand(4, 80))
+        q, s = quantize_rows(x)
+        for width, pitch in ((90, 112), (96, 97)):                                               # ... and int8 rows whose padding is not zero, or that begin on odd bytes
+            rows = torch.full((m, pitch), 99, device=DEV, dtype=torch.int8)
+            rows[:, :width] = q[:, :width]
+            assert torch.equal(linear_int8(rows[:, :width], padded[:, :width] if width == 90 else wq, ws, x_scale=s),
+                               linear_int8(q[:, :width].contiguous(), wq[:, :width].contiguous(), ws, x_scale=s))
     assert linear_int8(x[:0], wq, ws).shape == (0, 80)
 
 
