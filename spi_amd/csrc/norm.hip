@@ -4,8 +4,8 @@
 //   s = residual + scale * a(gate) * z      (the residual stream, rounded once to the row type)
 //   y = Norm(s) * pre_weight + pre_bias     (for the next block; from the UNROUNDED s), or its rows in 8 bits
 //
-// Bound by HBM: h and residual in, s and y out, once each.  A row stays in the registers of the threads that loaded it, so both norms' sums run over
-// registers; sums are fp32.
+// Bound by HBM: h and residual in, s and y out, once each (4 x 4096 x 2048 bf16: 72 us = 3.7 TB/s, where a copy of 1 GiB reaches 5.1).  A row stays in the registers of the threads that loaded it, so both norms' sums run over
+// registers; sums are fp32 (a row whose squares pass the fp32 range has a deviation of infinity, and is normalised to 0).
 #include "typed.hpp"
 #include <algorithm>
 
@@ -99,8 +99,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(const N
     const bool live = row_at < d.rows;                                         // (a dead row meets every barrier of its block, with another row's values)
     const int64_t row = live ? row_at : d.rows - 1, base = row * d.width, gbase = d.gate_mode ? gate_at(d, row) : 0;
     int phase = 0, at[NV], first[NV];
-    // (the gate and the weights are read where they are used: read ahead, or held for several rows, they cost so many registers that fewer rows are under way --
-    //  4 x 4096 x 2048 bf16: 60 us as it is, 79 and 68 us)
+    // (the gate and the weights are read where they are used.  4 x 4096 x 2048 bf16: 72 us; read ahead with the rows, 80: the registers cost rows under way.  Held in registers
+    //  while a block walks several rows, 69 -- but 8 x 600 x 1024 fp16 15.6 instead of 13.4, and fp32 3 x 667 x 1003 13.7 instead of 12.8.)
     Chunk<T, VEC> hc[NV], rc[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -225,8 +225,9 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int& ph
     }
 }
 
-// Bound by HBM (h, residual, ds, dy in; d_h, d_residual out) as far as enough of it is under way: a block holds few rows, so the rows of the next two turns are on their way
-// while one is worked on.  With one row ahead a CU has 32 KB under way and 4 x 4096 x 2048 bf16 takes 139 us (2.9 TB/s), with or without the sums between the threads.
+// Bound by HBM (h, residual, ds, dy in; d_h, d_residual out) as far as enough of it is under way: a block holds few rows, so the next row's values are on their way while a
+// row is worked on, in loads without a condition (a load under one is waited for at once).  4 x 4096 x 2048 bf16: 105 us = 3.8 TB/s; 139 us with conditional loads, with or
+// without the sums between the threads; 184 us without the next row.
 template <typename T, int VEC, int TPR, int NV, bool LAYER>
 __global__ void __launch_bounds__(TPR > BT ? TPR : BT, TPR > BT ? 4 : sizeof(T) == 4 && NV == 1 ? 3 : 2) norm_bwd_kernel(const NormBwdArgs a) {
     constexpr int G = TPR > BT ? 1 : BT / TPR;
@@ -272,8 +273,8 @@ __global__ void __launch_bounds__(TPR > BT ? TPR : BT, TPR > BT ? 4 : sizeof(T) 
         }
     };
     for (int64_t seg = blockIdx.x; seg < a.nseg; seg += gridDim.x) {
-        // G rows at a time, all segments of a sample side by side: blocks that each kept to rows of their own would all be at the same place of a 128 KB stride, on few of
-        // the memory's channels (4 x 4096 x 2048 bf16: 142 us)
+        // G rows at a time, all segments of a sample side by side, so that the blocks together read one run of memory (blocks that each kept to rows of their own, 128 KB
+        // apart: 4 % slower)
         const int64_t sample = seg / a.segs_per_sample, row0 = sample * a.sample_rows + seg % a.segs_per_sample * G, row1 = (sample + 1) * a.sample_rows;
         const int64_t stride = a.segs_per_sample * G;
         if (d.gate_mode && !full) {

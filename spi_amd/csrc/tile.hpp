@@ -210,8 +210,8 @@ struct TileEngine {
         const int steps = (int)((a.k + KT - 1) / KT);
         auto fetch = [&](char* to) { la.fetch(to); lb.fetch(to + BM * 128); };
         auto put = [&](char* to) { la.put(to); lb.put(to + BM * 128); };
-        // the fragments of part kk + 1 are read while part kk is multiplied
-        auto multiply = [&](const char* from) {
+        // the fragments of part kk + 1 are read while part kk is multiplied; the copies of the next step start behind the first fragments' reads
+        auto multiply = [&](const char* from, char* next) {
             i32x4_t fa[2][FM], fb[2][FN];
             auto read = [&](int kk) {
 #pragma unroll
@@ -220,6 +220,9 @@ struct TileEngine {
                 for (int j = 0; j < FN; ++j) fb[kk & 1][j] = rb.read(from + BM * 128, j, kk);
             };
             read(0);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(next);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) {
                 if (kk < 3) read(kk + 1);
@@ -236,9 +239,7 @@ struct TileEngine {
         // behind the barrier a stage is whole (it waits for this wave's copies, too) and nobody reads the other one any more; copies behind the last step read nothing
         auto step = [&](char* now, char* next) {
             __syncthreads();
-            fetch(next);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(now);
+            multiply(now, next);
             put(next);
         };
         fetch(s0);

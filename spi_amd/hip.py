@@ -181,23 +181,23 @@ DTYPE_I8 = 4
 
 
 def same_device(*tensors):
-    """The GPU that all given tensors (None: absent) live on; raises if there is a CPU tensor or a second device among them."""
+    """Index of the GPU that all given tensors (None: absent) live on; raises if there is a CPU tensor or a second device among them."""
     device = None
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError('spi_amd kernels need GPU tensors (no CPU fallback); got a %s tensor' % t.device.type)
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f'tensors on different devices: {device} and {t.device}')
+        if t is not None:
+            d = t.get_device()
+            if d != device:
+                if not t.is_cuda:
+                    raise RuntimeError('spi_amd kernels need GPU tensors (no CPU fallback); got a %s tensor' % t.device.type)
+                if device is not None:
+                    raise RuntimeError(f'tensors on different devices: cuda:{device} and cuda:{d}')
+                device = d
     return device
 
 
 def on(device, fn, *args):
-    """fn(*args) with `device` as the current one: launches go to ITS current stream, workspaces come from its memory."""
-    if device.index == torch.cuda.current_device():
+    """fn(*args) with the GPU `device` (an index) as the current one: launches go to ITS current stream, workspaces come from its memory."""
+    if device == torch.cuda.current_device():
         return fn(*args)
     with torch.cuda.device(device):
         return fn(*args)

@@ -44,7 +44,7 @@ class _GroupedLinear(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, offsets = ctx.saved_tensors
-        return (None, *hip.on(x.device, _backward, ctx.cfg, ctx.needs_input_grad[1:4], x, weight, offsets, dy), None)
+        return (None, *hip.on(x.get_device(), _backward, ctx.cfg, ctx.needs_input_grad[1:4], x, weight, offsets, dy), None)
 
 
 def _backward(cfg, need, x, weight, offsets, dy):

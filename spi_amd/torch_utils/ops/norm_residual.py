@@ -78,7 +78,7 @@ class _NormResidual(torch.autograd.Function):
             weights = weights[:2] + [None, None]
             need = need[:5] + (False, False)
         inputs = (h, residual, gate, *weights)
-        return (None, *hip.on(h.device, _backward, cfg, need, stats, inputs, d_stream, d_normed))
+        return (None, *hip.on(h.get_device(), _backward, cfg, need, stats, inputs, d_stream, d_normed))
 
 
 def _backward(cfg, need, stats, inputs, d_stream, d_normed):
@@ -105,16 +105,17 @@ def _backward(cfg, need, stats, inputs, d_stream, d_normed):
 
 def _gate_mode(h, gate):
     """-> (mode, rows that share a gate vector)"""
-    width, rows = h.shape[-1], h.numel() // h.shape[-1]
     if gate is None:
         return _GATE_NONE, 1
+    width = h.shape[-1]
     if gate.ndim >= 1 and gate.shape[-1] == width:
         if gate.numel() == width:
             return _GATE_CHANNEL, 1
         if gate.shape == h.shape:
             return _GATE_FULL, 1
         if h.ndim >= 3 and gate.shape[0] == h.shape[0] and gate.numel() == h.shape[0] * width and (gate.ndim == 2 or gate.ndim == h.ndim):
-            return (_GATE_SAMPLE, rows // h.shape[0]) if rows > h.shape[0] else (_GATE_FULL, 1)
+            rows = h.numel() // width // h.shape[0]
+            return (_GATE_SAMPLE, rows) if rows > 1 else (_GATE_FULL, 1)
     raise ValueError(f'gate {tuple(gate.shape)} is neither one vector of {width}, nor one for each sample, nor one value for each of {tuple(h.shape)}')
 
 
@@ -155,9 +156,10 @@ def norm_residual(h, residual, gate=None, scale=1.0, post_weight=None, post_bias
         raise TypeError(f'norm weights of {kind}: float32 or {h.dtype}')
     if gate is not None and gate.dtype is not h.dtype and gate.dtype is not torch.float32:
         raise TypeError(f'gate of {gate.dtype}: float32 or {h.dtype}')
+    vector = (width,)
     for t in weights:
         if t is not None:
-            if t.shape != (width,):
+            if t.shape != vector:
                 raise ValueError(f'a norm weight of {tuple(t.shape)} for rows of {width}')
             if t.dtype is not kind:
                 raise TypeError(f'norm weights of {kind} and {t.dtype}: one type for all')
@@ -173,7 +175,7 @@ def norm_residual(h, residual, gate=None, scale=1.0, post_weight=None, post_bias
         raise RuntimeError('norm_residual: rounded rows have no gradient; call quantize=True under torch.no_grad() or on tensors that need none')
     if wants_grad and width > MAX_WIDTH_BACKWARD:
         raise ValueError(f'rows of {width} values: gradients are provided up to {MAX_WIDTH_BACKWARD}')
-    h, residual, gate, *weights = [t if t is None or t.is_contiguous() else t.contiguous() for t in (h, residual, gate) + weights]
+    h, residual, gate, *weights = [t if t is None else t.contiguous() for t in (h, residual, gate) + weights]
     cfg = (h.numel() // width, width, per_sample, mode, _ba.activation_funcs[gate_act][0], norm == 'layer', after, before, float(scale), float(eps))
     if wants_grad:
         return hip.on(device, _NormResidual.apply, cfg, h, residual, gate, *weights)

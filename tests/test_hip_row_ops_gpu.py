@@ -460,11 +460,12 @@ def test_grouped_reads_offsets_as_running_maximum():
             assert torch.equal(u, v)
 
 
-def test_grouped_strides_and_rows_stand_alone():
+@pytest.mark.parametrize('k,n', [(96, 72), (99, 75)])
+def test_grouped_strides_and_rows_stand_alone(k, n):
     from spi_amd.torch_utils.ops.grouped_linear import grouped_linear
     g = gen(11)
     for dtype in TYPES:
-        x, w = randn(g, 150, 96, dtype=dtype), randn(g, 3, 72, 96, dtype=dtype)
+        x, w = randn(g, 150, k, dtype=dtype), randn(g, 3, n, k, dtype=dtype)
         o = torch.tensor([0, 20, 90, 150], device=DEV, dtype=torch.int32)
         want = grouped_linear(x, w, o)
         assert torch.equal(grouped_linear(x.t().contiguous().t(), w.transpose(1, 2).contiguous().transpose(1, 2), o), want)
@@ -472,7 +473,7 @@ def test_grouped_strides_and_rows_stand_alone():
         assert odd[0].data_ptr() % 16 and odd[1].data_ptr() % 16
         off = grouped_linear(*odd, o)
         r, mag = ref.grouped(x.double(), w.double(), None, o.tolist(), 1.0)
-        ref.check(off, r, mag, 2 * 96 + 8, 'rows on odd places')
+        ref.check(off, r, mag, 2 * k + 8, 'rows on odd places')
         bad = x.clone()
         bad[21, 7], bad[89, 0] = float('nan'), float('inf')
         y = grouped_linear(bad, w, o)
@@ -480,9 +481,40 @@ def test_grouped_strides_and_rows_stand_alone():
         assert torch.equal(y[keep], want[keep]) and torch.isnan(y[21]).all() and not torch.isfinite(y[89]).any()
         # ... and in the sums over a group's rows they reach that group's gradients only
         xg, wg = bad.clone().requires_grad_(), w.clone().requires_grad_()
-        dy = randn(g, 150, 72, dtype=dtype)
+        dy = randn(g, 150, n, dtype=dtype)
         _, dw = torch.autograd.grad(grouped_linear(xg, wg, o), [xg, wg], dy)
         assert torch.isfinite(dw[0]).all() and torch.isfinite(dw[2]).all() and torch.isnan(dw[1, :, 7]).all()
+        # a group's own weights, and gradients that come in, stay with their group and row, too
+        spoiled = w.clone()
+        spoiled[1, 3, 5] = float('nan')
+        y = grouped_linear(x, spoiled, o)
+        assert torch.equal(y[:20], want[:20]) and torch.equal(y[90:], want[90:]) and torch.isnan(y[20:90, 3]).all()
+        xg, wg, bg = x.clone().requires_grad_(), w.clone().requires_grad_(), randn(g, 3, n, dtype=dtype).requires_grad_()
+        first = torch.autograd.grad(grouped_linear(xg, wg, o, bias=bg), [xg, wg, bg], dy)
+        dy[95, 2] = float('nan')
+        second = torch.autograd.grad(grouped_linear(xg, wg, o, bias=bg), [xg, wg, bg], dy)
+        assert torch.equal(first[0][:95], second[0][:95]) and torch.equal(first[0][96:], second[0][96:]) and torch.isnan(second[0][95]).all()
+        assert all(torch.equal(first[i][:2], second[i][:2]) for i in (1, 2)) and torch.isnan(second[2][2, 2]) and torch.isfinite(second[2][2, 3:]).all()
+
+
+def test_grouped_rows_behind_32_bits():
+    from spi_amd.torch_utils.ops.grouped_linear import grouped_linear
+    t, k, n = 540_000, 4096, 16                                       # 2.2e9 values
+    g = gen(12)
+    x, dy = torch.zeros(t, k, device=DEV, dtype=BF16), torch.zeros(t, n, device=DEV, dtype=BF16)
+    x[-300:], dy[-300:] = randn(g, 300, k, dtype=BF16), randn(g, 300, n, dtype=BF16)
+    w = randn(g, 2, n, k, dtype=BF16).requires_grad_()
+    x.requires_grad_()
+    o = torch.tensor([0, t - 200, t], device=DEV, dtype=torch.int32)
+    y = grouped_linear(x, w, o, gain=0.1)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    offsets, xs, ds, ws = [0, 100, 300], x.detach()[-300:].double(), dy[-300:].double(), w.detach().double()
+    r, mag = ref.grouped(xs, ws, None, offsets, 0.1)
+    ref.check(y[-300:], r, mag, 2 * k + 8, 'y')
+    exact, mags = ref.grouped_gradients(xs, ws, offsets, 0.1, ds)
+    ref.check(dx[-300:], exact[0], mags[0], 2 * n + 8, 'dx')
+    ref.check(dw, exact[1], mags[1], 2 * 300 + 8, 'dw')               # (zeros before, which round nothing)
+    assert not y[:-300].any() and not dx[:-300].any()
 
 
 def test_grouped_gradients_match_differences():

@@ -66,7 +66,7 @@ def test_c_entries_return_errors():
     n.width = 64
     n.d_pre_weight = p
     assert L.spi_norm_residual_bwd_workspace(ctypes.byref(n)) > 0 and L.spi_norm_residual_bwd(ctypes.byref(n), None) == -1 and b'workspace' in L.spi_last_error()
-    i = hip.LinearInt8Desc(4, 8, 32, 0, 0, 32, 32, 256, p, None, p, p, None, p, 1, 0.0, 1.0, -1.0)
+    i = hip.LinearInt8Desc(40, 8, 32, 0, 0, 32, 32, 256, p, None, p, p, None, p, 1, 0.0, 1.0, -1.0)
     for field, value in (('M', -1), ('N', 0), ('K', 131072), ('x_dtype', 2), ('x_dtype', 4), ('y_dtype', 4), ('x_stride', 31), ('w_stride', 31), ('w_bytes', 255), ('act', 0), ('act', 10),
                          ('x', None), ('y', None), ('w', None), ('w_scale', None)):
         d = hip.LinearInt8Desc.from_buffer_copy(i)
