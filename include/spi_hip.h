@@ -536,7 +536,7 @@ int spi_adam_multi_dev(void* const* ptrs, const int64_t* sizes, int T, int64_t m
  *   Norm(x) = (x - m) / sqrt(mean((x - m)^2) + eps), m = mean(x) if `layer`, else 0;  a: SPI_ACT_LINEAR / _TANH / _SIGMOID
  * gate_mode 0 none, 1 [width], 2 [rows / rows_per_sample, width], 3 [rows, width].  Weights, biases and gate: fp32 or `dtype`; biases may be NULL.
  * q [rows, q_stride] with q_stride = width .. width rounded up to 16 (the padding is written as 0): q = rint(y / t), t = max|y| / 127 -> q_scale [rows].
- * stats [rows, 4] (mean and 1/deviation of both norms): written by _fwd if not NULL, read by _bwd.  width <= SPI_NORM_MAX_WIDTH, _bwd _MAX_WIDTH_BWD.
+ * stats [rows, 4] (mean and 1/deviation of both norms; begins on 16 bytes): written by _fwd if not NULL, read by _bwd.  width <= SPI_NORM_MAX_WIDTH, _bwd _MAX_WIDTH_BWD.
  * _bwd: d_stream (NULL = 0) and, if `before`, d_normed in; every other gradient pointer may be NULL (not wanted); weight and shared-gate gradients are sums
  * over rows in a fixed order.  rows >= 1; workspace: spi_norm_residual_bwd_workspace(d) bytes. */
 #define SPI_NORM_MAX_WIDTH 32768
@@ -567,7 +567,7 @@ int spi_norm_residual_bwd(const spi_norm_residual_desc* d, spi_stream_t stream);
 int spi_quantize_rows(const void* x, int64_t rows, int width, int64_t x_stride, int dtype, int8_t* q, int64_t q_stride, float* scale, spi_stream_t stream);
 
 /* y [M,N] = clamp(act(x_scale[m] * w_scale[n] * sum_k q[m,k] w[n,k] + bias[n]) * gain), the sum in 32-bit integers (exact: K <= SPI_LINEAR_INT8_MAX_K).  8-bit rows are at
- * most 2^22 bytes apart.
+ * most 2^22 bytes apart; M <= 2^30.
  * x: int8 rows (x_dtype = SPI_DTYPE_I8, x_scale given), or rows of fp32 / fp16 / bf16, which the call quantises as spi_quantize_rows does.
  * x rows x_stride elements, w rows w_stride bytes apart (any alignment; fastest where rows begin on 16 bytes); y contiguous, of type y_dtype; bias fp32 or NULL; act: any SPI_ACT_*.
  * w_bytes: bytes that may be read from w (>= (N-1) * w_stride + K).  workspace: spi_linear_int8_workspace(d) bytes. */
@@ -592,6 +592,7 @@ int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t stream);
 
 /* Products of ragged groups of rows: group e is the rows offsets[e] .. offsets[e+1]-1 of x [T,K] (offsets: E+1 int32 in DEVICE memory; read as their running
  * maximum, clamped to 0 .. T).  Contiguous tensors of one type (fp32, fp16, bf16), sums in fp32:
+ *   (T, E, N, K at most 2^30, 65535, 2^20, 2^20)
  *   _fwd:   y [T,N]     = gain * x W[e]^T + bias[e]      (W [E,N,K], bias [E,N] or NULL);  rows of no group: 0
  *   _dgrad: dx [T,K]    = gain * dy W[e];                                                  rows of no group: 0
  *   _wgrad: dw [E,N,K]  = gain * dy^T x over the group,  db [E,N] = column sums of dy;     either may be NULL; empty groups: 0

@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
     constexpr int VEC = Chunk<T>::N, G = 256 / TPR;
     __shared__ float red[4];
     const int t = threadIdx.x % TPR;
-    const int64_t row_at = (int64_t)blockIdx.x * G + threadIdx.x / TPR;
+    const int64_t row_at = row_block() * G + threadIdx.x / TPR;
     const bool live = row_at < rows;
     const int64_t row = live ? row_at : rows - 1;
     const T* p = x + row * x_stride;
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 
 template <typename T, int TPR, int NV>
 void launch_quantize(const void* x, int64_t rows, int width, int64_t x_stride, int8_t* q, int64_t q_stride, int room, float* scale, hipStream_t st) {
-    hipLaunchKernelGGL((quantize_rows_kernel<T, TPR, NV>), dim3((unsigned)ceil_div64(rows, 256 / TPR)), dim3(256), 0, st, (const T*)x, rows, width, x_stride, q, q_stride, room,
+    hipLaunchKernelGGL((quantize_rows_kernel<T, TPR, NV>), row_grid(ceil_div64(rows, 256 / TPR)), dim3(256), 0, st, (const T*)x, rows, width, x_stride, q, q_stride, room,
                        scale);
 }
 template <typename T>
@@ -291,8 +291,8 @@ void quantize_any(const void* x, int64_t rows, int width, int64_t x_stride, int 
 
 int check_int8(const spi_linear_int8_desc* d, const char* who) {
     SPI_REQUIRE(d, "%s: no descriptor", who);
-    SPI_REQUIRE(d->M >= 0 && d->M < (1ll << 31) - 64 && d->N >= 1 && d->K >= 1 && d->K <= SPI_LINEAR_INT8_MAX_K && ceil_div64(d->M, 64) * ceil_div64(d->N, 64) < (1ll << 31), "%s: M %lld, N %d, K %d", who,
-                (long long)d->M, d->N, d->K);
+    SPI_REQUIRE(d->M >= 0 && d->M <= (1ll << 30) && d->N >= 1 && d->K >= 1 && d->K <= SPI_LINEAR_INT8_MAX_K && ceil_div64(d->M, 64) * ceil_div64(d->N, 64) < (1ll << 31),
+                "%s: M %lld, N %d, K %d", who, (long long)d->M, d->N, d->K);
     SPI_REQUIRE(d->x_dtype == SPI_DTYPE_I8 || float_rows(d->x_dtype), "%s: x_dtype %d", who, d->x_dtype);
     SPI_REQUIRE(float_rows(d->y_dtype), "%s: y_dtype %d", who, d->y_dtype);
     SPI_REQUIRE(d->M == 0 || (d->x && d->y), "%s: null rows", who);
@@ -496,7 +496,7 @@ void grouped_pass(int dtype, const GroupArgs& a, hipStream_t st) {
 }
 int check_grouped(const spi_grouped_linear_desc* d, const char* who) {
     SPI_REQUIRE(d, "%s: no descriptor", who);
-    SPI_REQUIRE(d->T >= 0 && d->T < (1ll << 31) - 64 && d->E >= 1 && d->E <= 65535 && d->N >= 1 && d->N <= (1 << 20) && d->K >= 1 && d->K <= (1 << 20),
+    SPI_REQUIRE(d->T >= 0 && d->T <= (1ll << 30) && d->E >= 1 && d->E <= 65535 && d->N >= 1 && d->N <= (1 << 20) && d->K >= 1 && d->K <= (1 << 20),
                 "%s: T %lld, E %d, N %d, K %d", who, (long long)d->T, d->E, d->N, d->K);
     SPI_REQUIRE((most_tiles(d->T, d->E, 64) * (int64_t)ceil_div64(std::max(d->N, d->K), 64) < (1ll << 31) - 1024) && ceil_div64(d->N, 64) * ceil_div64(d->K, 64) * d->E < (1ll << 31) - 1024,
                 "%s: T %lld, E %d, N %d, K %d are more tiles than a launch has blocks", who, (long long)d->T, d->E, d->N, d->K);

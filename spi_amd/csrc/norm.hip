@@ -4,8 +4,9 @@
 //   s = residual + scale * a(gate) * z      (the residual stream, rounded once to the row type)
 //   y = Norm(s) * pre_weight + pre_bias     (for the next block; from the UNROUNDED s), or its rows in 8 bits
 //
-// Bound by HBM: h and residual in, s and y out, once each (4 x 4096 x 2048 bf16: 72 us = 3.7 TB/s, where a copy of 1 GiB reaches 5.1).  A row stays in the registers of the threads that loaded it, so both norms' sums run over
-// registers; sums are fp32 (a row whose squares pass the fp32 range has a deviation of infinity, and is normalised to 0).
+// Bound by HBM: h and residual in, s and y out, once each (4 x 4096 x 2048 bf16: 72 us = 3.7 TB/s, where a copy of 1 GiB reaches 5.1).  A row stays in the
+// registers of the threads that loaded it, so both norms' sums run over registers; sums are fp32 (a row whose squares pass the fp32 range has a deviation of
+// infinity, and is normalised to 0).
 #include "typed.hpp"
 #include <algorithm>
 
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) norm_fwd_kernel(const N
     __shared__ float red[32];
     const spi_norm_residual_desc& d = a.d;
     const int t = threadIdx.x % TPR;
-    const int64_t row_at = (int64_t)blockIdx.x * G + threadIdx.x / TPR;
+    const int64_t row_at = row_block() * G + threadIdx.x / TPR;
     const bool live = row_at < d.rows;                                         // (a dead row meets every barrier of its block, with another row's values)
     const int64_t row = live ? row_at : d.rows - 1, base = row * d.width, gbase = d.gate_mode ? gate_at(d, row) : 0;
     int phase = 0, at[NV], first[NV];
@@ -508,26 +509,30 @@ int check_desc(const spi_norm_residual_desc* d, const char* who) {
     SPI_REQUIRE(!d->after || d->post_weight, "%s: null post_weight", who);
     SPI_REQUIRE(!d->before || d->pre_weight, "%s: null pre_weight", who);
     SPI_REQUIRE(d->eps > 0.f, "%s: eps %g", who, (double)d->eps);
+    SPI_REQUIRE(((uintptr_t)d->stats & 15) == 0, "%s: stats do not begin on 16 bytes", who);
     return SPI_OK;
 }
 
 template <typename T, int VEC, int TPR, int NV>
 void launch_fwd(const NormArgs& a, hipStream_t st) {
     constexpr int THREADS = TPR > 256 ? TPR : 256;
-    const dim3 grid((unsigned)ceil_div64(a.d.rows, THREADS / TPR));
+    const dim3 grid = row_grid(ceil_div64(a.d.rows, THREADS / TPR));
     if (a.d.layer) hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, TPR, NV, true>), grid, dim3(THREADS), 0, st, a);
     else hipLaunchKernelGGL((norm_fwd_kernel<T, VEC, TPR, NV, false>), grid, dim3(THREADS), 0, st, a);
 }
+// One chunk a thread as far as a block goes: the latency of a row is what few rows cost, and many rows hide it either way.  One chunk / two in half the threads:
+// 1 x 512 fp32 3.1 / 3.8 us, 8 x 600 x 1024 fp16 13.7 / 14.3, 2 x 4096 bf16 4.1 / 4.8, 4000 x 4096 bf16 35.8 / 36.1; two / four: 1 x 8000 fp16 6.5 / 9.2,
+// 2000 x 8000 40.3 / 40.4.
 template <typename T>
 void dispatch_fwd(const NormArgs& a, hipStream_t st) {
     constexpr int N = Chunk<T>::N;
     const int chunks = (int)ceil_div64(a.d.width, N);
     if (a.d.width < N) launch_fwd<T, 1, 64, 1>(a, st);
     else if (chunks <= 64) launch_fwd<T, N, 64, 1>(a, st);
-    else if (chunks <= 128) launch_fwd<T, N, 64, 2>(a, st);
+    else if (chunks <= 128) launch_fwd<T, N, 128, 1>(a, st);
     else if (chunks <= 256) launch_fwd<T, N, 256, 1>(a, st);
-    else if (chunks <= 512) launch_fwd<T, N, 256, 2>(a, st);
-    else if (chunks <= 1024) launch_fwd<T, N, 256, 4>(a, st);
+    else if (chunks <= 512) launch_fwd<T, N, 512, 1>(a, st);
+    else if (chunks <= 1024) launch_fwd<T, N, 512, 2>(a, st);
     else if (chunks <= 2048) launch_fwd<T, N, 1024, 2>(a, st);
     else if (sizeof(T) < 4 || chunks <= 4096) launch_fwd<T, N, 1024, 4>(a, st);       // (SPI_NORM_MAX_WIDTH is 4096 chunks of eight)
     else if constexpr (sizeof(T) == 4) launch_fwd<T, N, 1024, 8>(a, st);

@@ -258,6 +258,23 @@ def test_norm_rows_behind_32_bits():
     assert torch.equal(s[-3:], last[0]) and torch.equal(y[-3:], last[1]) and not s[:-3].any() and not y[:-3].any()
 
 
+def test_more_narrow_rows_than_a_launch_has_threads():
+    from spi_amd.torch_utils.ops.linear_int8 import quantize_rows
+    rows = (1 << 26) + 5                                            # a wave each: more than 2^32 lanes
+    x = torch.zeros(rows, 2, device=DEV, dtype=F16)
+    x[-7:], x[:3] = randn(gen(4), 7, 2, dtype=F16), 1
+    w = torch.ones(2, device=DEV)
+    i = dict(h=x, residual=x, gate=None, post_weight=w, post_bias=None, pre_weight=w, pre_bias=None)
+    s, y = run_norm(i, 0.5, 'rms', 'both', 1e-6, 'linear')
+    q, scale = quantize_rows(x)
+    for part in (slice(0, 9), slice(rows - 9, rows)):
+        few = x[part].clone()
+        fs, fy = run_norm({**i, 'h': few, 'residual': few}, 0.5, 'rms', 'both', 1e-6, 'linear')
+        fq, fscale = quantize_rows(few)
+        assert torch.equal(s[part], fs) and torch.equal(y[part], fy) and torch.equal(q[part], fq) and torch.equal(scale[part], fscale) and fs.any()
+    assert not s[3:-7].any() and not y[3:-7].any() and not scale[3:-7].any()
+
+
 # ---- 8-bit integers ----------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('dtype', TYPES, ids=ids)
 @pytest.mark.parametrize('rows,width', [(1, 1), (3, 15), (7, 512), (2, 1003), (33, 2048), (5, 8192), (2, 100_001)])

@@ -57,7 +57,7 @@ def test_c_entries_return_errors():
     p = 0x1000
     n = hip.NormResidualDesc(4, 1, 64, 0, 0, 0, 0, 1, 0, 1, 1, 1.0, 1e-6, p, p, None, p, None, p, None)
     for field, value in (('width', 0), ('width', 32769), ('dtype', 2), ('weight_dtype', 1), ('gate_mode', 1), ('gate_mode', 9), ('gate_act', 3), ('eps', 0.0), ('h', None),
-                         ('pre_weight', None), ('rows', -1), ('rows', 1 << 31), ('stream_out', None)):
+                         ('pre_weight', None), ('rows', -1), ('rows', 1 << 31), ('stream_out', None), ('stats', p + 8)):
         d = hip.NormResidualDesc.from_buffer_copy(n)
         setattr(d, field, value)
         assert L.spi_norm_residual_fwd(ctypes.byref(d), None) == -1 and L.spi_last_error(), field
@@ -67,7 +67,7 @@ def test_c_entries_return_errors():
     n.d_pre_weight = p
     assert L.spi_norm_residual_bwd_workspace(ctypes.byref(n)) > 0 and L.spi_norm_residual_bwd(ctypes.byref(n), None) == -1 and b'workspace' in L.spi_last_error()
     i = hip.LinearInt8Desc(40, 8, 32, 0, 0, 32, 32, 256, p, None, p, p, None, p, 1, 0.0, 1.0, -1.0)
-    for field, value in (('M', -1), ('N', 0), ('K', 131072), ('x_dtype', 2), ('x_dtype', 4), ('y_dtype', 4), ('x_stride', 31), ('w_stride', 31), ('w_bytes', 255), ('act', 0), ('act', 10),
+    for field, value in (('M', -1), ('M', (1 << 30) + 1), ('N', 0), ('K', 131072), ('x_dtype', 2), ('x_dtype', 4), ('y_dtype', 4), ('x_stride', 31), ('w_stride', 31), ('w_bytes', 255), ('act', 0), ('act', 10),
                          ('x', None), ('y', None), ('w', None), ('w_scale', None)):
         d = hip.LinearInt8Desc.from_buffer_copy(i)
         setattr(d, field, value)
