@@ -108,8 +108,10 @@ template <int SIZE, int LOAD>
 __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) int8_tile_kernel(const Int8Args a, int rows, int cols) {
     typedef Engine<int8_t, SIZE, false, false, LOAD> E;
     __shared__ __attribute__((aligned(1024))) char s0[E::STAGE], s1[E::STAGE];
+    const int64_t block = row_block();
+    if (block >= rows * cols) return;                                          // (rows * cols < 2^31, see check_int8)
     int row, col;
-    band_order(xcd_run(blockIdx.x, gridDim.x), rows, cols, row, col);
+    band_order(xcd_run((int)block, rows * cols), rows, cols, row, col);
     const int m0 = row * SIZE, n0 = col * SIZE, m = min(SIZE, a.M - m0), n = min(SIZE, a.N - n0);
     typename E::Accs acc = {};
     const int64_t k = LOAD == LOAD_DMA ? (a.K + 15) / 16 * 16 : a.K;           // (LOAD_DMA: the padding of the quantised rows is 0, so that of the weights does not count)
@@ -139,7 +141,10 @@ __global__ void __launch_bounds__(256) int8_few_rows_kernel(const Int8Args a, co
     __shared__ float scales[FEW], red[2][4];
     __shared__ int part[4][FEW][FEW + 1];
     constexpr int N = Chunk<T>::N;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pitch = few_pitch(a.K), n0 = blockIdx.x * FEW;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, pitch = few_pitch(a.K);
+    const int64_t block = row_block();
+    if (block * FEW >= a.N) return;
+    const int n0 = (int)block * FEW;
     if constexpr (sizeof(T) == 1) {
         const int whole = a.K / 16, rest = pitch / 16 - whole;
 #pragma unroll 4
@@ -309,7 +314,7 @@ bool few_rows(const spi_linear_int8_desc& d) { return d.M <= FEW && d.M * few_pi
 bool few_floats(const spi_linear_int8_desc& d) { return few_rows(d) && d.M <= FEW_FLOATS && d.x_dtype != SPI_DTYPE_I8; }
 template <typename T>
 void launch_few(const spi_linear_int8_desc& d, const Int8Args& a, const void* x, int64_t x_stride, hipStream_t st) {
-    hipLaunchKernelGGL(int8_few_rows_kernel<T>, dim3((unsigned)ceil_div64(d.N, FEW)), dim3(256), (size_t)d.M * few_pitch(d.K), st, a, (const T*)x, x_stride, d.w_bytes);
+    hipLaunchKernelGGL(int8_few_rows_kernel<T>, row_grid(ceil_div64(d.N, FEW)), dim3(256), (size_t)d.M * few_pitch(d.K), st, a, (const T*)x, x_stride, d.w_bytes);
 }
 
 // ---- ragged groups -----------------------------------------------------------------------------------------------------------------------
@@ -376,9 +381,10 @@ __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) grouped_tile_kernel(c
     __shared__ __attribute__((aligned(1024))) char s0[E::STAGE], s1[E::STAGE];
     const int width = PASS == PASS_FWD ? a.N : a.K, cols = (width + SIZE - 1) / SIZE;
     const int rows = PASS == PASS_WGRAD ? (a.N + SIZE - 1) / SIZE : count_tiles(a.offsets, a.E, a.T, SIZE), tiles = rows * cols * (PASS == PASS_WGRAD ? a.E : 1);
-    const int whole = SIZE == 256 ? whole_tiles(tiles) : tiles, cut = (int)blockIdx.x - whole;
-    const int tile = cut < 0 ? (int)blockIdx.x : whole + cut / 4;
-    if (tile >= tiles) return;
+    const int64_t block = row_block();
+    const int whole = SIZE == 256 ? whole_tiles(tiles) : tiles;
+    if (block >= (SIZE == 256 ? whole + (int64_t)(tiles - whole) * 4 : tiles)) return;
+    const int cut = (int)(block - whole), tile = cut < 0 ? (int)block : whole + cut / 4;
     int row, col, r0 = 0;
     RowTile t;
     if constexpr (PASS == PASS_WGRAD) {
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(256) grouped_bias_grad_kernel(const GroupArgs 
 }
 template <typename T>
 __global__ void __launch_bounds__(256) grouped_bias_join_kernel(const GroupArgs a, const float* __restrict__ part, int S) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = row_block() * 256 + threadIdx.x;
     if (i >= (int64_t)a.E * a.N) return;
     const float* p = part + i / a.N * S * a.N + i % a.N;
     float v = 0.f;
@@ -450,7 +456,7 @@ template <typename T, int VEC>
 void bias_grad(const spi_grouped_linear_desc& d, const GroupArgs& a, hipStream_t st) {
     const int S = bias_parts(d);
     hipLaunchKernelGGL((grouped_bias_grad_kernel<T, VEC>), dim3((unsigned)ceil_div64(d.N, 64 * VEC), (unsigned)S, (unsigned)d.E), dim3(256), 0, st, a, (float*)d.workspace, S);
-    if (S > 1) hipLaunchKernelGGL(grouped_bias_join_kernel<T>, dim3((unsigned)ceil_div64((int64_t)d.E * d.N, 256)), dim3(256), 0, st, a, (const float*)d.workspace, S);
+    if (S > 1) hipLaunchKernelGGL(grouped_bias_join_kernel<T>, row_grid(ceil_div64((int64_t)d.E * d.N, 256)), dim3(256), 0, st, a, (const float*)d.workspace, S);
 }
 template <typename T>
 void bias_grad(const spi_grouped_linear_desc& d, const GroupArgs& a, hipStream_t st) {
@@ -471,7 +477,7 @@ int tile_edge(F rows, int64_t width, bool dma) {
 template <typename T, int PASS, int SIZE, int LOAD>
 void launch_tiles(const GroupArgs& a, hipStream_t st) {
     const int64_t tiles = PASS == PASS_WGRAD ? ceil_div64(a.N, SIZE) * ceil_div64(a.K, SIZE) * a.E : most_tiles(a.T, a.E, SIZE) * ceil_div64(PASS == PASS_FWD ? a.N : a.K, SIZE);
-    hipLaunchKernelGGL((grouped_tile_kernel<T, PASS, SIZE, LOAD>), dim3((unsigned)(SIZE == 256 ? most_blocks(tiles) : tiles)), dim3(SIZE == 256 ? 512 : 256), 0, st, a);
+    hipLaunchKernelGGL((grouped_tile_kernel<T, PASS, SIZE, LOAD>), row_grid(SIZE == 256 ? most_blocks(tiles) : tiles), dim3(SIZE == 256 ? 512 : 256), 0, st, a);
 }
 template <typename T, int PASS>
 void grouped_pass(const GroupArgs& a, hipStream_t st) {
@@ -555,7 +561,7 @@ extern "C" int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t strea
     const bool dma = aligned16(a.q) && aligned16(a.w) && a.q_stride % 16 == 0 && a.w_stride % 16 == 0 &&
                      (d->K % 16 == 0 || (d->x_dtype != SPI_DTYPE_I8 && d->w_bytes >= (int64_t)(d->N - 1) * d->w_stride + q_pitch(d->K)));
     const int size = tile_edge([&](int edge) { return ceil_div64(d->M, edge); }, d->N, dma), rows = (int)ceil_div64(d->M, size), cols = (int)ceil_div64(d->N, size);
-    const dim3 grid((unsigned)rows * (unsigned)cols);
+    const dim3 grid = row_grid((int64_t)rows * cols);
     if (size == 256) hipLaunchKernelGGL((int8_tile_kernel<256, LOAD_DMA>), grid, dim3(512), 0, st, a, rows, cols);
     else if (size == 128 && dma) hipLaunchKernelGGL((int8_tile_kernel<128, LOAD_DMA>), grid, dim3(256), 0, st, a, rows, cols);
     else if (size == 128) hipLaunchKernelGGL((int8_tile_kernel<128, LOAD_WIDE>), grid, dim3(256), 0, st, a, rows, cols);

@@ -150,8 +150,8 @@ __device__ __forceinline__ Chunk<int8_t, N> quantize_values(const float (&v)[N],
     for (int j = 0; j < N; ++j) q.v[j] = (int8_t)(int)r[j];
     return q;
 }
-// n blocks as a grid of two axes, for kernels whose blocks take rows: along one axis a launch has less than 2^32 threads (here: 2^31 in blocks of 1024).
-// The blocks behind n have no rows.
+// n blocks as a grid of two axes, for kernels whose blocks take rows or tiles: along one axis a launch has less than 2^32 threads (here: 2^31 in blocks of 1024).
+// The blocks behind n have no work.
 inline dim3 row_grid(int64_t n) {
     const int64_t x = n < (1 << 21) ? n : 1 << 21;
     return dim3((unsigned)x, (unsigned)ceil_div64(n, x));
