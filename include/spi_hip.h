@@ -30,7 +30,7 @@ typedef void* spi_stream_t;           /* hipStream_t */
 #define SPI_ERR_UNSUPPORTED -2        /* valid request this build has no kernel for */
 #define SPI_ERR_LAUNCH      -3        /* hipGetLastError() != hipSuccess after the launch */
 
-#define SPI_ABI_VERSION 14   /* 2: spi_raymarch_bwd gained d_color_scale, spi_triplane_decode_bwd_sorted gained d_rgb_scale
+#define SPI_ABI_VERSION 15   /* 2: spi_raymarch_bwd gained d_color_scale, spi_triplane_decode_bwd_sorted gained d_rgb_scale
                              * 3: spi_conv_desc gained workspace / workspace_bytes (Winograd path), spi_conv2d_workspace_bytes
                              * 4: + spi_sample_from_planes_fwd / _bwd (additive)
                              * 5: + contextual / roi_align / adam_pred / filtered_lrelu_fused   6: + spi_affine_fwd / _bwd   7: + spi_decoder_gains (additive)
@@ -42,7 +42,8 @@ typedef void* spi_stream_t;           /* hipStream_t */
                              *     SPI_DTYPE_F64 for spi_bias_act_t / spi_upfirdn2d_t (additive)
                              * 12: + spi_tail_bwd_dot_t (additive); spi_conv2d_workspace_bytes / workspace of fp16 activation tensors select the direct fp16 kernels
                              * 13: + spi_conv_wino_f4_set (additive); the Winograd workspace of a >= 256^2 layer is 2.25x larger (36 instead of 16 frequencies)
-                             * 14: + spi_norm_residual_fwd / _bwd, spi_quantize_rows, spi_linear_int8, spi_grouped_linear_fwd / _dgrad / _wgrad, SPI_DTYPE_BF16 / _I8 (additive) */
+                             * 14: + spi_norm_residual_fwd / _bwd, spi_quantize_rows, spi_linear_int8, spi_grouped_linear_fwd / _dgrad / _wgrad, SPI_DTYPE_BF16 / _I8 (additive)
+                             * 15: + spi_linear_int8_tile, spi_grouped_linear_tile (additive) */
 int         spi_abi_version(void);
 int         spi_sizeof_conv_desc(void);   /* sizeof(spi_conv_desc) of THIS build: bindings assert it against their own struct */
 const char* spi_last_error(void);     /* thread-local, valid until the next failing call */
@@ -586,7 +587,12 @@ typedef struct spi_linear_int8_desc {
     void* workspace;
     int64_t workspace_bytes;
 } spi_linear_int8_desc;
+/* The matrix tile that a product takes, decided on the host from sizes, strides and alignment (the pointers are not read): its edge (64, 128, 256) | its loader << 16;
+ * 0: no tile (up to 16 rows have a kernel of their own, no rows none at all); < 0: an error.
+ * _COPY: memory -> LDS as the rows lie, rows begin and end on 16 bytes; _WIDE: 16 bytes at a time at any alignment, operands have 16 bytes at least; _EACH: value by value. */
+enum { SPI_TILE_COPY = 0, SPI_TILE_WIDE = 1, SPI_TILE_EACH = 2 };
 int spi_sizeof_linear_int8_desc(void);
+int spi_linear_int8_tile(const spi_linear_int8_desc* d);
 int64_t spi_linear_int8_workspace(const spi_linear_int8_desc* d);
 int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t stream);
 
@@ -610,6 +616,7 @@ typedef struct spi_grouped_linear_desc {
     int64_t workspace_bytes;
 } spi_grouped_linear_desc;
 int spi_sizeof_grouped_linear_desc(void);
+int spi_grouped_linear_tile(const spi_grouped_linear_desc* d, int pass);     /* as spi_linear_int8_tile */
 int64_t spi_grouped_linear_workspace(const spi_grouped_linear_desc* d, int pass);
 int spi_grouped_linear_fwd(const spi_grouped_linear_desc* d, spi_stream_t stream);
 int spi_grouped_linear_dgrad(const spi_grouped_linear_desc* d, spi_stream_t stream);

@@ -312,6 +312,16 @@ int check_int8(const spi_linear_int8_desc* d, const char* who) {
 int64_t q_pitch(int K) { return ceil_div64(K, 16) * 16; }
 bool few_rows(const spi_linear_int8_desc& d) { return d.M <= FEW && d.M * few_pitch(d.K) <= FEW_LDS; }
 bool few_floats(const spi_linear_int8_desc& d) { return few_rows(d) && d.M <= FEW_FLOATS && d.x_dtype != SPI_DTYPE_I8; }
+// rows of floats: as they lie in the workspace once they are quantised, the scales behind them
+Int8Args int8_args(const spi_linear_int8_desc& d) {
+    Int8Args a{(const int8_t*)d.x, d.x_scale, d.w, d.w_scale, d.bias, d.y, d.x_stride, d.w_stride, (int)d.M, d.N, d.K, d.y_dtype, d.act, d.alpha, d.gain, d.clamp};
+    if (d.x_dtype != SPI_DTYPE_I8) {
+        a.q = (const int8_t*)d.workspace;
+        a.q_stride = q_pitch(d.K);
+        a.q_scale = (const float*)(a.q + d.M * a.q_stride);
+    }
+    return a;
+}
 template <typename T>
 void launch_few(const spi_linear_int8_desc& d, const Int8Args& a, const void* x, int64_t x_stride, hipStream_t st) {
     hipLaunchKernelGGL(int8_few_rows_kernel<T>, row_grid(ceil_div64(d.N, FEW)), dim3(256), (size_t)d.M * few_pitch(d.K), st, a, (const T*)x, x_stride, d.w_bytes);
@@ -469,10 +479,27 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // more.  Measured, bf16 forward, edges 64 / 128 / 256: 2048 x 1024 x 1024 in 4 groups (144 tiles of 128) 11.4 / 15.8 / 15.5 us, 8192 x 1024 x 1024 in 8 (544, 128 of 256)
 // 32.5 / 25.2 / 31.6, 16384 x 2048 x 2048 in 8 (512 of 256) 307 / 206 / 196; int8 4096^3 (256 of 256) 130 / 105 / 94.  Through registers (rows on odd places) 128 pays later:
 // bf16 weight gradient of 8192 x 1003 x 501 (256 tiles of 128) 37 / 55.
+struct Tile { int edge, load; };
+// rows(edge): tile rows at that edge; smallest: bytes of the smaller operand, from its first value to its tensor's end.  Rows that cannot be copied to LDS as they lie are read 16
+// bytes at a time, which takes operands of 16 bytes at least -- whatever the edge, and for a sum over nothing, too: the first step's loads come before the count of steps.
 template <typename F>
-int tile_edge(F rows, int64_t width, bool dma) {
-    if (dma && rows(256) * ceil_div64(width, 256) >= CUS) return 256;
-    return rows(128) * ceil_div64(width, 128) >= (dma ? CUS : CUS * 3 / 2) ? 128 : 64;
+Tile choose_tile(F rows, int64_t width, bool dma, int64_t smallest) {
+    if (!dma && smallest < 16) return Tile{64, LOAD_EACH};
+    if (dma && rows(256) * ceil_div64(width, 256) >= CUS) return Tile{256, LOAD_DMA};
+    return Tile{rows(128) * ceil_div64(width, 128) >= (dma ? CUS : CUS * 3 / 2) ? 128 : 64, dma ? LOAD_DMA : LOAD_WIDE};
+}
+Tile choose_int8(const spi_linear_int8_desc& d, const Int8Args& a) {
+    // 16-byte rows; where they do not end on 16 bytes, the rows' own padding has to be 0 and the weights' readable
+    const bool dma = aligned16(a.q) && aligned16(a.w) && a.q_stride % 16 == 0 && a.w_stride % 16 == 0 &&
+                     (d.K % 16 == 0 || (d.x_dtype != SPI_DTYPE_I8 && d.w_bytes >= (d.N - 1) * d.w_stride + q_pitch(d.K)));
+    return choose_tile([&](int edge) { return ceil_div64(d.M, edge); }, d.N, dma, std::min((d.M - 1) * a.q_stride, (d.N - 1) * a.w_stride) + d.K);
+}
+Tile choose_grouped(const spi_grouped_linear_desc& d, int pass) {
+    const int64_t es = d.dtype == SPI_DTYPE_F32 ? 4 : 2, xs = d.T * d.K, ws = (int64_t)d.E * d.N * d.K, ds = d.T * d.N;
+    const bool dma = d.N * es % 16 == 0 && d.K * es % 16 == 0 && aligned16(d.x) && aligned16(d.w) && aligned16(d.dy);
+    const int64_t smallest = (pass == PASS_FWD ? std::min(xs, ws) : pass == PASS_DGRAD ? std::min(ds, ws) : std::min(ds, xs)) * es;
+    auto rows = [&](int edge) { return pass == PASS_WGRAD ? ceil_div64(d.N, edge) * d.E : d.T / edge + std::min<int64_t>(d.T, d.E) / 2; };      // (of ragged groups half a tile each is empty)
+    return choose_tile(rows, pass == PASS_FWD ? d.N : d.K, dma, smallest);
 }
 template <typename T, int PASS, int SIZE, int LOAD>
 void launch_tiles(const GroupArgs& a, hipStream_t st) {
@@ -480,25 +507,20 @@ void launch_tiles(const GroupArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((grouped_tile_kernel<T, PASS, SIZE, LOAD>), row_grid(SIZE == 256 ? most_blocks(tiles) : tiles), dim3(SIZE == 256 ? 512 : 256), 0, st, a);
 }
 template <typename T, int PASS>
-void grouped_pass(const GroupArgs& a, hipStream_t st) {
-    constexpr int ES = (int)sizeof(T);
-    const bool dma = a.N * ES % 16 == 0 && a.K * ES % 16 == 0 && aligned16(a.x) && aligned16(a.w) && aligned16(a.dy);
-    const int64_t width = PASS == PASS_FWD ? a.N : a.K;
-    auto rows = [&](int size) { return PASS == PASS_WGRAD ? ceil_div64(a.N, size) * a.E : a.T / size + std::min(a.T, a.E) / 2; };        // (of ragged groups half a tile each is empty)
-    const int size = tile_edge(rows, width, dma);
-    const int64_t smallest = std::min({(int64_t)a.T * a.K, (int64_t)a.T * a.N, (int64_t)a.E * a.N * a.K}) * ES;
-    if (size == 256) launch_tiles<T, PASS, 256, LOAD_DMA>(a, st);
-    else if (size == 128 && dma) launch_tiles<T, PASS, 128, LOAD_DMA>(a, st);
-    else if (size == 128) launch_tiles<T, PASS, 128, LOAD_WIDE>(a, st);
-    else if (dma) launch_tiles<T, PASS, 64, LOAD_DMA>(a, st);
-    else if (smallest >= 16) launch_tiles<T, PASS, 64, LOAD_WIDE>(a, st);
+void grouped_pass(const GroupArgs& a, Tile t, hipStream_t st) {
+    if (t.edge == 256) launch_tiles<T, PASS, 256, LOAD_DMA>(a, st);
+    else if (t.edge == 128 && t.load == LOAD_DMA) launch_tiles<T, PASS, 128, LOAD_DMA>(a, st);
+    else if (t.edge == 128) launch_tiles<T, PASS, 128, LOAD_WIDE>(a, st);
+    else if (t.load == LOAD_DMA) launch_tiles<T, PASS, 64, LOAD_DMA>(a, st);
+    else if (t.load == LOAD_WIDE) launch_tiles<T, PASS, 64, LOAD_WIDE>(a, st);
     else launch_tiles<T, PASS, 64, LOAD_EACH>(a, st);
 }
 template <int PASS>
-void grouped_pass(int dtype, const GroupArgs& a, hipStream_t st) {
-    if (dtype == SPI_DTYPE_F32) grouped_pass<float, PASS>(a, st);
-    else if (dtype == SPI_DTYPE_F16) grouped_pass<half_t, PASS>(a, st);
-    else grouped_pass<bf16_t, PASS>(a, st);
+void grouped_pass(const spi_grouped_linear_desc& d, const GroupArgs& a, hipStream_t st) {
+    const Tile t = choose_grouped(d, PASS);
+    if (d.dtype == SPI_DTYPE_F32) grouped_pass<float, PASS>(a, t, st);
+    else if (d.dtype == SPI_DTYPE_F16) grouped_pass<half_t, PASS>(a, t, st);
+    else grouped_pass<bf16_t, PASS>(a, t, st);
 }
 int check_grouped(const spi_grouped_linear_desc* d, const char* who) {
     SPI_REQUIRE(d, "%s: no descriptor", who);
@@ -532,12 +554,18 @@ extern "C" int64_t spi_linear_int8_workspace(const spi_linear_int8_desc* d) {
     if (check_int8(d, "spi_linear_int8_workspace") || d->x_dtype == SPI_DTYPE_I8 || few_floats(*d)) return 0;
     return d->M * (q_pitch(d->K) + (int64_t)sizeof(float));
 }
+extern "C" int spi_linear_int8_tile(const spi_linear_int8_desc* d) {
+    if (int rc = check_int8(d, "spi_linear_int8_tile")) return rc;
+    if (d->M == 0 || few_rows(*d)) return 0;
+    const Tile t = choose_int8(*d, int8_args(*d));
+    return t.edge | t.load << 16;
+}
 extern "C" int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t stream) {
     if (int rc = check_int8(d, "spi_linear_int8")) return rc;
     if (d->M == 0) return SPI_OK;
     SPI_REQUIRE(d->workspace_bytes >= spi_linear_int8_workspace(d) && (d->workspace || d->workspace_bytes == 0), "spi_linear_int8: workspace too small");
     hipStream_t st = as_stream(stream);
-    Int8Args a{(const int8_t*)d->x, d->x_scale, d->w, d->w_scale, d->bias, d->y, d->x_stride, d->w_stride, (int)d->M, d->N, d->K, d->y_dtype, d->act, d->alpha, d->gain, d->clamp};
+    const Int8Args a = int8_args(*d);
     if (few_floats(*d)) {
         if (d->x_dtype == SPI_DTYPE_F32) launch_few<float>(*d, a, d->x, d->x_stride, st);
         else if (d->x_dtype == SPI_DTYPE_F16) launch_few<half_t>(*d, a, d->x, d->x_stride, st);
@@ -546,9 +574,6 @@ extern "C" int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t strea
         return SPI_OK;
     }
     if (d->x_dtype != SPI_DTYPE_I8) {
-        a.q = (int8_t*)d->workspace;
-        a.q_stride = q_pitch(d->K);
-        a.q_scale = (float*)((char*)d->workspace + d->M * a.q_stride);
         quantize_any(d->x, d->M, d->K, d->x_stride, d->x_dtype, (int8_t*)a.q, a.q_stride, (float*)a.q_scale, st);
         SPI_LAUNCH_CHECK("spi_linear_int8 (quantize)");
     }
@@ -557,16 +582,14 @@ extern "C" int spi_linear_int8(const spi_linear_int8_desc* d, spi_stream_t strea
         SPI_LAUNCH_CHECK("spi_linear_int8");
         return SPI_OK;
     }
-    // 16-byte rows; where they do not end on 16 bytes, the rows' own padding has to be 0 and the weights' readable
-    const bool dma = aligned16(a.q) && aligned16(a.w) && a.q_stride % 16 == 0 && a.w_stride % 16 == 0 &&
-                     (d->K % 16 == 0 || (d->x_dtype != SPI_DTYPE_I8 && d->w_bytes >= (int64_t)(d->N - 1) * d->w_stride + q_pitch(d->K)));
-    const int size = tile_edge([&](int edge) { return ceil_div64(d->M, edge); }, d->N, dma), rows = (int)ceil_div64(d->M, size), cols = (int)ceil_div64(d->N, size);
+    const Tile t = choose_int8(*d, a);
+    const int rows = (int)ceil_div64(d->M, t.edge), cols = (int)ceil_div64(d->N, t.edge);
     const dim3 grid = row_grid((int64_t)rows * cols);
-    if (size == 256) hipLaunchKernelGGL((int8_tile_kernel<256, LOAD_DMA>), grid, dim3(512), 0, st, a, rows, cols);
-    else if (size == 128 && dma) hipLaunchKernelGGL((int8_tile_kernel<128, LOAD_DMA>), grid, dim3(256), 0, st, a, rows, cols);
-    else if (size == 128) hipLaunchKernelGGL((int8_tile_kernel<128, LOAD_WIDE>), grid, dim3(256), 0, st, a, rows, cols);
-    else if (dma) hipLaunchKernelGGL((int8_tile_kernel<64, LOAD_DMA>), grid, dim3(256), 0, st, a, rows, cols);
-    else if ((d->M - 1) * a.q_stride + d->K >= 16 && (d->N - 1) * a.w_stride + d->K >= 16) hipLaunchKernelGGL((int8_tile_kernel<64, LOAD_WIDE>), grid, dim3(256), 0, st, a, rows, cols);
+    if (t.edge == 256) hipLaunchKernelGGL((int8_tile_kernel<256, LOAD_DMA>), grid, dim3(512), 0, st, a, rows, cols);
+    else if (t.edge == 128 && t.load == LOAD_DMA) hipLaunchKernelGGL((int8_tile_kernel<128, LOAD_DMA>), grid, dim3(256), 0, st, a, rows, cols);
+    else if (t.edge == 128) hipLaunchKernelGGL((int8_tile_kernel<128, LOAD_WIDE>), grid, dim3(256), 0, st, a, rows, cols);
+    else if (t.load == LOAD_DMA) hipLaunchKernelGGL((int8_tile_kernel<64, LOAD_DMA>), grid, dim3(256), 0, st, a, rows, cols);
+    else if (t.load == LOAD_WIDE) hipLaunchKernelGGL((int8_tile_kernel<64, LOAD_WIDE>), grid, dim3(256), 0, st, a, rows, cols);
     else hipLaunchKernelGGL((int8_tile_kernel<64, LOAD_EACH>), grid, dim3(256), 0, st, a, rows, cols);
     SPI_LAUNCH_CHECK("spi_linear_int8");
     return SPI_OK;
@@ -578,12 +601,19 @@ extern "C" int64_t spi_grouped_linear_workspace(const spi_grouped_linear_desc* d
     const int S = bias_parts(*d);
     return S > 1 ? (int64_t)d->E * S * d->N * (int64_t)sizeof(float) : 0;
 }
+extern "C" int spi_grouped_linear_tile(const spi_grouped_linear_desc* d, int pass) {
+    if (int rc = check_grouped(d, "spi_grouped_linear_tile")) return rc;
+    SPI_REQUIRE(pass >= PASS_FWD && pass <= PASS_WGRAD, "spi_grouped_linear_tile: pass %d", pass);
+    if (d->T == 0 && pass != PASS_WGRAD) return 0;
+    const Tile t = choose_grouped(*d, pass);
+    return t.edge | t.load << 16;
+}
 extern "C" int spi_grouped_linear_fwd(const spi_grouped_linear_desc* d, spi_stream_t stream) {
     if (int rc = check_grouped(d, "spi_grouped_linear_fwd")) return rc;
     if (d->T == 0) return SPI_OK;
     SPI_REQUIRE(d->x && d->w && d->y, "spi_grouped_linear_fwd: null pointer");
     const GroupArgs a = group_args(*d);
-    grouped_pass<PASS_FWD>(d->dtype, a, as_stream(stream));
+    grouped_pass<PASS_FWD>(*d, a, as_stream(stream));
     SPI_LAUNCH_CHECK("spi_grouped_linear_fwd");
     return SPI_OK;
 }
@@ -592,7 +622,7 @@ extern "C" int spi_grouped_linear_dgrad(const spi_grouped_linear_desc* d, spi_st
     if (d->T == 0) return SPI_OK;
     SPI_REQUIRE(d->dy && d->w && d->dx, "spi_grouped_linear_dgrad: null pointer");
     const GroupArgs a = group_args(*d);
-    grouped_pass<PASS_DGRAD>(d->dtype, a, as_stream(stream));
+    grouped_pass<PASS_DGRAD>(*d, a, as_stream(stream));
     SPI_LAUNCH_CHECK("spi_grouped_linear_dgrad");
     return SPI_OK;
 }
@@ -602,7 +632,7 @@ extern "C" int spi_grouped_linear_wgrad(const spi_grouped_linear_desc* d, spi_st
     SPI_REQUIRE(d->T == 0 || !d->dw || d->x, "spi_grouped_linear_wgrad: null x");
     const GroupArgs a = group_args(*d);
     if (d->dw) {
-        grouped_pass<PASS_WGRAD>(d->dtype, a, as_stream(stream));
+        grouped_pass<PASS_WGRAD>(*d, a, as_stream(stream));
         SPI_LAUNCH_CHECK("spi_grouped_linear_wgrad");
     }
     if (d->db) {

@@ -57,8 +57,9 @@ __device__ __forceinline__ int row_swizzle(int r) { return (r & 7) ^ ((r >> 3) &
 //   LOAD_WIDE  through registers (`fetch` before a step's products, `put` behind them), 16 bytes at a time at any alignment, without a condition -- a load under a condition
 //              would be waited for at once.  A chunk that would pass the tensor's end is read from its last 16 bytes and moved into place by `put`, which also clears what lies
 //              behind the summed axis
-//   LOAD_EACH  value by value where a tensor has less than 16 bytes
-enum { LOAD_DMA, LOAD_WIDE, LOAD_EACH };
+//              behind the summed axis.  The tensor has 16 bytes at least
+//   LOAD_EACH  value by value where a tensor has less than 16 bytes, or none
+enum { LOAD_DMA = SPI_TILE_COPY, LOAD_WIDE = SPI_TILE_WIDE, LOAD_EACH = SPI_TILE_EACH };
 template <typename T, int R, int NW, bool COL, int LOAD>
 struct TileLoader {
     static constexpr int ES = (int)sizeof(T), KT = 128 / ES, PER = R / 8 / NW, ROW = COL ? R * ES : 128, RPI = 1024 / ROW, CHUNKS = ROW / 16;

@@ -11,7 +11,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libspi_hip.so')
 _lib = None
-ABI_VERSION = 14          # SPI_ABI_VERSION of include/spi_hip.h this binding was written against
+ABI_VERSION = 15          # SPI_ABI_VERSION of include/spi_hip.h this binding was written against
 
 c_f = ctypes.c_float
 c_i = ctypes.c_int
@@ -136,9 +136,11 @@ _SIGS = {
     'spi_quantize_rows': ([c_p, c_l, c_i, c_l, c_i, c_p, c_l, c_p, c_p], c_i),
     'spi_sizeof_linear_int8_desc': ([], c_i),
     'spi_linear_int8_workspace': ([ctypes.POINTER(LinearInt8Desc)], c_l),
+    'spi_linear_int8_tile': ([ctypes.POINTER(LinearInt8Desc)], c_i),
     'spi_linear_int8': ([ctypes.POINTER(LinearInt8Desc), c_p], c_i),
     'spi_sizeof_grouped_linear_desc': ([], c_i),
     'spi_grouped_linear_workspace': ([ctypes.POINTER(GroupedLinearDesc), c_i], c_l),
+    'spi_grouped_linear_tile': ([ctypes.POINTER(GroupedLinearDesc), c_i], c_i),
     'spi_grouped_linear_fwd': ([ctypes.POINTER(GroupedLinearDesc), c_p], c_i),
     'spi_grouped_linear_dgrad': ([ctypes.POINTER(GroupedLinearDesc), c_p], c_i),
     'spi_grouped_linear_wgrad': ([ctypes.POINTER(GroupedLinearDesc), c_p], c_i),
