@@ -538,8 +538,9 @@ int spi_adam_multi_dev(void* const* ptrs, const int64_t* sizes, int T, int64_t m
  * gate_mode 0 none, 1 [width], 2 [rows / rows_per_sample, width], 3 [rows, width].  Weights, biases and gate: fp32 or `dtype`; biases may be NULL.
  * q [rows, q_stride] with q_stride = width .. width rounded up to 16 (the padding is written as 0): q = rint(y / t), t = max|y| / 127 -> q_scale [rows].
  * stats [rows, 4] (mean and 1/deviation of both norms; begins on 16 bytes): written by _fwd if not NULL, read by _bwd.  width <= SPI_NORM_MAX_WIDTH, _bwd _MAX_WIDTH_BWD.
- * _bwd: d_stream (NULL = 0) and, if `before`, d_normed in; every other gradient pointer may be NULL (not wanted); weight and shared-gate gradients are sums
- * over rows in a fixed order.  rows >= 1; workspace: spi_norm_residual_bwd_workspace(d) bytes. */
+ * _bwd: d_stream (NULL = 0) and, if `before`, d_normed in; a pass in which normed has no part says before = 0, also where `after` is 0 and no norm is left.  Every other
+ * gradient pointer may be NULL (not wanted); weight and shared-gate gradients are sums over rows in a fixed order.  rows >= 1; workspace: spi_norm_residual_bwd_workspace(d)
+ * bytes. */
 #define SPI_NORM_MAX_WIDTH 32768
 #define SPI_NORM_MAX_WIDTH_BWD 8192
 typedef struct spi_norm_residual_desc {

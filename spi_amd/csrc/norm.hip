@@ -502,7 +502,6 @@ int check_desc(const spi_norm_residual_desc* d, const char* who) {
     auto param_ok = [&](int t) { return t == SPI_DTYPE_F32 || t == d->dtype; };
     SPI_REQUIRE(param_ok(d->weight_dtype) && param_ok(d->gate_dtype), "%s: weights / gate are fp32 or of the rows' type", who);
     SPI_REQUIRE(d->h && d->residual, "%s: null rows", who);
-    SPI_REQUIRE(d->after || d->before, "%s: no norm", who);
     SPI_REQUIRE(d->gate_mode >= GATE_NONE && d->gate_mode <= GATE_FULL && (d->gate_mode == GATE_NONE) == (d->gate == nullptr), "%s: gate and gate_mode disagree", who);
     SPI_REQUIRE(d->gate_mode != GATE_SAMPLE || (d->rows_per_sample >= 1 && d->rows % d->rows_per_sample == 0), "%s: rows_per_sample %lld", who, (long long)d->rows_per_sample);
     SPI_REQUIRE(d->gate_act == SPI_ACT_LINEAR || d->gate_act == SPI_ACT_TANH || d->gate_act == SPI_ACT_SIGMOID, "%s: gate_act %d", who, d->gate_act);
@@ -558,6 +557,7 @@ void dispatch_bwd(const NormBwdArgs& a, const BwdPlan& p, hipStream_t st) {
 
 extern "C" int spi_norm_residual_fwd(const spi_norm_residual_desc* d, spi_stream_t stream) {
     if (int rc = check_desc(d, "spi_norm_residual_fwd")) return rc;
+    SPI_REQUIRE(d->after || d->before, "spi_norm_residual_fwd: no norm");
     SPI_REQUIRE(d->stream_out, "spi_norm_residual_fwd: null stream_out");
     SPI_REQUIRE(!d->before || (d->q ? (d->q_scale && d->q_stride >= d->width) : d->normed != nullptr), "spi_norm_residual_fwd: no place for the normed rows");
     // (a row's threads cover at least its chunks: the padding that they write as 0 ends with the last chunk, at most 15 bytes behind the row)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import row_ops_ref as ref
-from test_hip_row_ops_gpu import check_grouped, int8_reference
+from test_hip_row_ops_gpu import ORDER, check_grouped, int8_reference, norm_case, norm_inputs, piled, run_norm
 
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
@@ -72,3 +72,55 @@ def test_linear_int8_with_weights_of_less_than_16_bytes(m, n, k):
         r, mag = int8_reference(q, s, wq, ws, None, 'lrelu', 2 ** 0.5, None)
         ref.check(linear_int8(x, wq, ws, act='lrelu'), r, mag, 8, f'{m} x {n} x {k}')
         ref.check(linear_int8(q.contiguous(), wq, ws, x_scale=s, act='lrelu'), r, mag, 8, f'{m} x {n} x {k} integers')
+
+
+# ---- gradients of a part of the results, for a part of the leaves ------------------------------------------------------------------------
+def check_part(inputs, norm, where, act, use, wanted, scale=-0.7, eps=1e-6):
+    """gradients of the results in ``use`` ('stream', 'normed') for the leaves in ``wanted``, against the 64-bit statement's.  A result without a use counts as one whose
+    gradient is 0; a leaf that is only behind such a result gets none."""
+    h = inputs['h']
+    v = {k: t if t is None else t.clone().requires_grad_(k in wanted) for k, t in inputs.items()}
+    results = dict(zip(('stream', 'normed'), run_norm(v, scale, norm, where, eps, act)))
+    ct = {k: randn(gen(i), *h.shape, dtype=h.dtype) if k in use else torch.zeros_like(h) for i, k in enumerate(('stream', 'normed'))}
+    leaves = [k for k in inputs if k in wanted and inputs[k] is not None]
+    got = torch.autograd.grad([results[k] for k in use], [v[k] for k in leaves], [ct[k] for k in use], allow_unused=True)
+    wide = {k: t if t is None else t.detach().double().requires_grad_() for k, t in inputs.items()}
+    exact = dict(zip(('stream', 'normed'), ref.norm_residual(*[scale if k == 'scale' else wide[k] for k in ORDER], norm, where, eps, act)))
+    exact = torch.autograd.grad([exact[k] for k in use], [wide[k] for k in leaves], [ct[k].double() for k in use], allow_unused=True)
+    mag = norm_case(inputs, scale, norm, where, eps, act, ct['stream'], None if where == 'after' else ct['normed'])
+    for k, a, e in zip(leaves, got, exact):
+        what = f'{norm} {where} {use} d_{k} of {wanted}'
+        if e is None:
+            assert a is None, what
+            continue
+        m, add = mag[k], 0
+        if a.shape != h.shape:                                        # a sum over rows
+            m = m.sum((0, 1)) if a.ndim == 1 else m.sum(1, keepdim=a.ndim == 3)
+            add = h.numel() // h.shape[-1]
+        assert a.shape == inputs[k].shape and a.dtype == inputs[k].dtype, what
+        ref.check(a, e, m, 4 * piled(h.shape[-1]) + add, what)
+
+
+@pytest.mark.parametrize('gate,act', [(None, 'linear'), ('channel', 'tanh'), ('sample', 'sigmoid'), ('sample2', 'linear'), ('full', 'tanh')])
+@pytest.mark.parametrize('where', ['both', 'before', 'after'])
+def test_norm_gradients_of_one_result(where, gate, act):
+    """the last block of a stack hands on its stream alone, a head reads the normed rows alone"""
+    for norm, dtype, wdtype in (('rms', F32, F32), ('layer', F16, F16), ('layer', BF16, F32)):
+        i = norm_inputs((3, 5, 200), dtype, norm, where, gate, True, wdtype=wdtype)
+        for use in (('stream',), ('normed',), ('stream', 'normed')):
+            if where != 'after' or 'normed' not in use:
+                check_part(i, norm, where, act, use, tuple(i))
+
+
+@pytest.mark.parametrize('shape', [(2, 3, 7), (1, 1, 512), (2, 700, 64), (2, 2, 2048), (1, 3, 4101), (2, 2, 8192)])
+def test_norm_gradients_of_the_stream_in_every_width(shape):
+    for dtype in (F32, BF16):
+        check_part(norm_inputs(shape, dtype, 'rms', 'before', 'sample', False), 'rms', 'before', 'linear', ('stream',), ('h', 'residual', 'gate'))
+
+
+@pytest.mark.parametrize('where', ['both', 'before', 'after'])
+def test_norm_gradients_of_one_leaf(where):
+    for norm, gate, act, dtype in (('rms', 'channel', 'tanh', F32), ('layer', 'sample', 'sigmoid', BF16), ('layer', 'full', 'linear', F16)):
+        i = norm_inputs((4, 9, 136), dtype, norm, where, gate, True)
+        for leaf in (k for k, t in i.items() if t is not None):
+            check_part(i, norm, where, act, ('stream',) if where == 'after' else ('stream', 'normed'), (leaf,))
