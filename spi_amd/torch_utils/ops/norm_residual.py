@@ -113,8 +113,8 @@ def _gate_mode(h, gate):
             return _GATE_CHANNEL, 1
         if gate.shape == h.shape:
             return _GATE_FULL, 1
-        if h.ndim >= 3 and gate.shape[0] == h.shape[0] and gate.numel() == h.shape[0] * width and (gate.ndim == 2 or gate.ndim == h.ndim):
-            rows = h.numel() // width // h.shape[0]
+        if h.ndim >= 3 and gate.shape[0] == h.shape[0] and gate.shape[1:-1].numel() == 1 and (gate.ndim == 2 or gate.ndim == h.ndim):
+            rows = h.shape[1:-1].numel()
             return (_GATE_SAMPLE, rows) if rows > 1 else (_GATE_FULL, 1)
     raise ValueError(f'gate {tuple(gate.shape)} is neither one vector of {width}, nor one for each sample, nor one value for each of {tuple(h.shape)}')
 

@@ -124,3 +124,17 @@ def test_norm_gradients_of_one_leaf(where):
         i = norm_inputs((4, 9, 136), dtype, norm, where, gate, True)
         for leaf in (k for k, t in i.items() if t is not None):
             check_part(i, norm, where, act, ('stream',) if where == 'after' else ('stream', 'normed'), (leaf,))
+
+
+@pytest.mark.parametrize('h,gate', [((0, 5, 64), (0, 1, 64)), ((0, 5, 64), (0, 64)), ((0, 5, 64), (0, 5, 64)), ((0, 5, 64), (64,)), ((2, 0, 64), (2, 1, 64)), ((0, 64), (0, 64))])
+def test_norm_of_an_empty_batch_with_every_gate(h, gate):
+    from spi_amd.torch_utils.ops.norm_residual import norm_residual
+    leaves = [torch.ones(s, device=DEV, requires_grad=True) for s in (h, h, gate, 64, 64)]
+    for kw in (dict(), dict(norm='layer', gate_act='tanh')):
+        s, y = norm_residual(leaves[0], leaves[1], gate=leaves[2], post_weight=leaves[3], pre_weight=leaves[4], **kw)
+        assert s.shape == y.shape == h
+        for v, g in zip(leaves, torch.autograd.grad(s.sum() + y.sum(), leaves)):
+            assert g.shape == v.shape and not g.any()
+        with torch.no_grad():
+            s, (q, scale) = norm_residual(leaves[0], leaves[1], gate=leaves[2], post_weight=leaves[3], pre_weight=leaves[4], quantize=True, **kw)
+        assert q.shape == h and scale.shape == h[:-1]

@@ -1,8 +1,11 @@
-"""What the row operators decide on the host beyond their refusals: which descriptors their C entries take."""
+"""What the row operators decide on the host, beyond their refusals: which descriptors their C entries take, how a gate lies over the rows, which calls record a derivative."""
 import ctypes
 
+import pytest
+import torch
 
 from spi_amd import hip
+from spi_amd.torch_utils.ops import norm_residual
 
 P = 0x1000                                                             # never read
 
@@ -16,3 +19,17 @@ def test_backward_takes_a_pass_in_which_no_norm_is_left():
     assert L.spi_norm_residual_bwd(ctypes.byref(d), None) == -1 and b'workspace' in L.spi_last_error()
     d.stream_out = P
     assert L.spi_norm_residual_fwd(ctypes.byref(d), None) == -1 and b'no norm' in L.spi_last_error()
+
+
+@pytest.mark.parametrize('h,gate,mode', [((0, 5, 8), (0, 1, 8), (2, 5)), ((0, 5, 8), (0, 8), (2, 5)), ((0, 5, 8), (0, 5, 8), (3, 1)), ((0, 5, 8), (8,), (1, 1)), ((2, 0, 8), (2, 1, 8), (3, 1)),
+                                         ((0, 8), (0, 8), (3, 1)), ((2, 5, 8), (2, 1, 8), (2, 5)), ((2, 3, 5, 8), (2, 8), (2, 15)), ((2, 1, 8), (2, 8), (3, 1)), ((1, 5, 8), (1, 1, 8), (1, 1))])
+def test_gates_of_empty_batches(h, gate, mode):
+    assert norm_residual._gate_mode(torch.zeros(h), torch.zeros(gate)) == mode
+    with pytest.raises(RuntimeError, match='GPU'):                     # a legal call but for its device
+        norm_residual.norm_residual(torch.zeros(h), torch.zeros(h), gate=torch.zeros(gate), post_weight=torch.zeros(8), pre_weight=torch.zeros(8))
+
+
+@pytest.mark.parametrize('h,gate', [((0, 5, 8), (0, 3, 8)), ((0, 5, 8), (0, 0, 8)), ((0, 5, 8), (1, 5, 8)), ((2, 0, 8), (3, 8)), ((2, 5, 8), (2, 5, 1, 8))])
+def test_gates_that_do_not_fit_an_empty_batch(h, gate):
+    with pytest.raises(ValueError, match='neither'):
+        norm_residual._gate_mode(torch.zeros(h), torch.zeros(gate))
