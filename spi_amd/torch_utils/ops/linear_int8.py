@@ -29,11 +29,13 @@ def _stride(x):
 def quantize_rows(x):
     """x [..., K] (fp32 / fp16 / bf16) -> (q int8 [..., K], scale fp32 [...]): ``scale = max|row| / 127``, ``q = round(row / scale)``, ties to even, the division in
     fp32.  A row of zeros has scale 0; a row that holds an infinity or NaN has scale NaN (so its products are NaN) and q = 0.  The rows of q begin on 16 bytes:
-    q is a view of a buffer with K rounded up to 16."""
+    q is a view of a buffer with K rounded up to 16.  Inference only: a call that would have to record a gradient raises."""
     if x.ndim < 1 or not 1 <= x.shape[-1] <= MAX_IN_FEATURES:
         raise ValueError(f'rows of {tuple(x.shape)[-1:]} values: 1 to {MAX_IN_FEATURES}')
     if x.dtype not in hip.ROW_DTYPES:
         raise TypeError(f'rows of {x.dtype}: float32, float16 or bfloat16')
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError('quantize_rows: rounded rows have no gradient; call it under torch.no_grad() or on tensors that need none')
     return hip.on(hip.same_device(x), _quantize, x)
 
 
@@ -42,7 +44,7 @@ def _quantize(x):
     pitch = (k + 15) // 16 * 16
     q = torch.empty(x.shape[:-1] + (pitch,), device=x.device, dtype=torch.int8)
     scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    r = _rows(x.detach())
+    r = _rows(x)
     hip.call('spi_quantize_rows', r.data_ptr(), r.shape[0], k, _stride(r), hip.ROW_DTYPES[x.dtype], q.data_ptr(), pitch, scale.data_ptr(), hip.stream())
     return (q if pitch == k else q[..., :k]), scale
 

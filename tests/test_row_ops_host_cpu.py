@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from spi_amd import hip
-from spi_amd.torch_utils.ops import norm_residual
+from spi_amd.torch_utils.ops import linear_int8, norm_residual
 
 P = 0x1000                                                             # never read
 
@@ -33,3 +33,12 @@ def test_gates_of_empty_batches(h, gate, mode):
 def test_gates_that_do_not_fit_an_empty_batch(h, gate):
     with pytest.raises(ValueError, match='neither'):
         norm_residual._gate_mode(torch.zeros(h), torch.zeros(gate))
+
+
+def test_quantize_rows_loses_no_gradient():
+    x = torch.zeros(3, 8, requires_grad=True)
+    with pytest.raises(RuntimeError, match='no gradient'):
+        linear_int8.quantize_rows(x)
+    for legal in (lambda: linear_int8.quantize_rows(x.detach()), torch.no_grad()(lambda: linear_int8.quantize_rows(x))):
+        with pytest.raises(RuntimeError, match='GPU'):                 # but for its device
+            legal()
