@@ -7,6 +7,7 @@ loaded, or a tensor is not a contiguous fp32 GPU tensor, the call raises.
 import ctypes
 import os
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'csrc', 'libspi_hip.so')
@@ -195,6 +196,19 @@ def same_device(*tensors):
                     raise RuntimeError(f'tensors on different devices: cuda:{device} and cuda:{d}')
                 device = d
     return device
+
+
+def records(*tensors):
+    """Whether a call on these tensors (None: absent) has to record a derivative: one of them requires a gradient, or carries a forward-mode tangent."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
 
 
 def on(device, fn, *args):

@@ -83,9 +83,10 @@ def grouped_linear(x, weight, offsets, bias=None, gain=1.0):
     if bias is not None and bias.shape != weight.shape[:2]:
         raise ValueError(f'bias {tuple(bias.shape)} for weights {tuple(weight.shape)}')
     device = hip.same_device(x, weight, offsets, bias)
+    wants_grad = hip.records(x, weight, bias)                          # (forward-mode tangents end in an error of the autograd function, which has none)
     x, weight, offsets = x.contiguous(), weight.contiguous(), offsets.contiguous()
     bias = None if bias is None else bias.contiguous()
     cfg = (x.shape[0], weight.shape[0], weight.shape[1], x.shape[1], hip.ROW_DTYPES[x.dtype], float(gain))
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+    if wants_grad:
         return hip.on(device, _GroupedLinear.apply, cfg, x, weight, bias, offsets)
     return hip.on(device, _forward, cfg, x, weight, bias, offsets)

@@ -34,7 +34,7 @@ def quantize_rows(x):
         raise ValueError(f'rows of {tuple(x.shape)[-1:]} values: 1 to {MAX_IN_FEATURES}')
     if x.dtype not in hip.ROW_DTYPES:
         raise TypeError(f'rows of {x.dtype}: float32, float16 or bfloat16')
-    if torch.is_grad_enabled() and x.requires_grad:
+    if hip.records(x):
         raise RuntimeError('quantize_rows: rounded rows have no gradient; call it under torch.no_grad() or on tensors that need none')
     return hip.on(hip.same_device(x), _quantize, x)
 
@@ -83,7 +83,7 @@ def linear_int8(x, weight_q, weight_scale, bias=None, x_scale=None, act='linear'
     out_dtype = out_dtype or (torch.float32 if int_rows else x.dtype)
     if out_dtype not in hip.ROW_DTYPES:
         raise TypeError(f'out_dtype {out_dtype}: float32, float16 or bfloat16')
-    if torch.is_grad_enabled() and (x.requires_grad or weight_scale.requires_grad or (bias is not None and bias.requires_grad) or (int_rows and x_scale.requires_grad)):
+    if hip.records(x, weight_scale, bias, x_scale):
         raise RuntimeError('linear_int8: rounded rows have no gradient; call it under torch.no_grad() or on tensors that need none')
     return hip.on(hip.same_device(x, weight_q, weight_scale, bias, x_scale), _linear, x, weight_q, weight_scale, bias, x_scale, act_id, float(d_alpha if alpha is None else alpha),
                   float(d_gain if gain is None else gain), float(-1 if clamp is None else clamp), out_dtype)

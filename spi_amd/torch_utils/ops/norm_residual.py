@@ -165,12 +165,7 @@ def norm_residual(h, residual, gate=None, scale=1.0, post_weight=None, post_bias
                 raise TypeError(f'norm weights of {kind} and {t.dtype}: one type for all')
     mode, per_sample = _gate_mode(h, gate)
     device = hip.same_device(h, residual, gate, *weights)
-    wants_grad = False
-    if torch.is_grad_enabled():
-        for t in (h, residual, gate) + weights:
-            if t is not None and t.requires_grad:
-                wants_grad = True
-                break
+    wants_grad = hip.records(h, residual, gate, *weights)             # (forward-mode tangents end in an error of the autograd function, which has none)
     if wants_grad and quantize:
         raise RuntimeError('norm_residual: rounded rows have no gradient; call quantize=True under torch.no_grad() or on tensors that need none')
     if wants_grad and width > MAX_WIDTH_BACKWARD:

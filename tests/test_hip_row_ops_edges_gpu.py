@@ -138,3 +138,25 @@ def test_norm_of_an_empty_batch_with_every_gate(h, gate):
         with torch.no_grad():
             s, (q, scale) = norm_residual(leaves[0], leaves[1], gate=leaves[2], post_weight=leaves[3], pre_weight=leaves[4], quantize=True, **kw)
         assert q.shape == h and scale.shape == h[:-1]
+
+
+def test_forward_mode_tangents_are_refused():
+    """no operator has a forward-mode derivative: a call on a tensor with a tangent raises, as bias_act's does, with and without gradients recorded, and loses nothing silently"""
+    from torch.autograd import forward_ad
+    from spi_amd.torch_utils.ops import bias_act, grouped_linear, linear_int8, norm_residual
+    g = gen(30)
+    x, w, vec = randn(g, 6, 16), randn(g, 2, 8, 16), randn(g, 16)
+    o = torch.tensor([0, 2, 6], device=DEV, dtype=torch.int32)
+    wq, ws = linear_int8.quantize_rows(randn(g, 8, 16))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: bias_act.bias_act(dual(x), act='lrelu'), lambda: norm_residual.norm_residual(dual(x), x, post_weight=vec, pre_weight=vec),
+                 lambda: norm_residual.norm_residual(x, x, gate=dual(vec), post_weight=vec, pre_weight=vec, quantize=True),
+                 lambda: norm_residual.norm_residual(x, x, pre_weight=dual(vec), where='before'), lambda: grouped_linear.grouped_linear(dual(x), w, o),
+                 lambda: grouped_linear.grouped_linear(x, dual(w), o), lambda: linear_int8.linear_int8(dual(x), wq, ws), lambda: linear_int8.quantize_rows(dual(x))]
+        for call in calls + [torch.no_grad()(c) for c in calls]:
+            with pytest.raises(RuntimeError):                          # (NotImplementedError, where an autograd function has no such rule, is one)
+                call()
+        want = norm_residual.norm_residual(x, x, post_weight=vec, pre_weight=vec)       # ... and tensors without one are served as ever
+    for a, b in zip(want, norm_residual.norm_residual(x, x, post_weight=vec, pre_weight=vec)):
+        assert torch.equal(a, b)

@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from spi_amd import hip
 from spi_amd.torch_utils.ops import linear_int8, norm_residual
@@ -42,3 +43,20 @@ def test_quantize_rows_loses_no_gradient():
     for legal in (lambda: linear_int8.quantize_rows(x.detach()), torch.no_grad()(lambda: linear_int8.quantize_rows(x))):
         with pytest.raises(RuntimeError, match='GPU'):                 # but for its device
             legal()
+
+
+def test_which_calls_record_a_derivative():
+    plain, leaf = torch.zeros(3, 8), torch.zeros(3, 8, requires_grad=True)
+    assert not hip.records() and not hip.records(plain, None) and hip.records(plain, None, leaf) and hip.records(leaf * 2)
+    with torch.no_grad():
+        assert not hip.records(leaf)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(plain, torch.ones(3, 8))
+        assert hip.records(None, dual) and not hip.records(plain) and not hip.records(torch.zeros(3, 8, dtype=torch.int8))
+        with torch.no_grad():                                          # (which has no say in forward mode)
+            assert hip.records(dual[:, :4])
+        for call in (lambda: linear_int8.quantize_rows(dual), lambda: linear_int8.linear_int8(dual, torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4)),
+                     torch.no_grad()(lambda: linear_int8.linear_int8(plain, torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4), bias=dual[0, :4]))):
+            with pytest.raises(RuntimeError, match='no gradient'):
+                call()
+    assert not hip.records(dual)
