@@ -1,5 +1,7 @@
 """GPU tests of the row operators (norm_residual, quantize_rows / linear_int8, grouped_linear) at the edges of what their calls take: the largest launches, every tile of the
 product kernels, empty and tiny operands, partial gradients.  The 64-bit statements and bounds are those of row_ops_ref."""
+import ctypes
+
 import pytest
 import torch
 
@@ -160,3 +162,98 @@ def test_forward_mode_tangents_are_refused():
         want = norm_residual.norm_residual(x, x, post_weight=vec, pre_weight=vec)       # ... and tensors without one are served as ever
     for a, b in zip(want, norm_residual.norm_residual(x, x, post_weight=vec, pre_weight=vec)):
         assert torch.equal(a, b)
+
+
+# ---- every tile of the product kernels -----------------------------------------------------------------------------------------------------
+# Small whole numbers: every product and every partial sum is exact in 32 bits, so a result is the exact one rounded once, whatever the order of the sum -- the tolerance is 0, and a
+# value that is lost, taken twice or from a wrong place shows.
+COPY, WIDE, EACH = range(3)
+
+
+def whole(g, *shape, dtype=F32, most=2):
+    return torch.randint(-most, most + 1, shape, device=DEV, generator=g).to(dtype)
+
+
+def grouped_tiles(x, w, dy, offsets):
+    from spi_amd import hip
+    t, k = x.shape
+    e, n = w.shape[:2]
+    tiles = []
+    for which, ptrs in enumerate(((x, w, None), (None, w, dy), (x, None, dy))):
+        px, pw, pd = (None if v is None else v.data_ptr() for v in ptrs)
+        d = hip.GroupedLinearDesc(t, e, n, k, hip.ROW_DTYPES[x.dtype], 1.0, px, pw, None, offsets.data_ptr())
+        d.dy = pd
+        code = hip.lib().spi_grouped_linear_tile(ctypes.byref(d), which)
+        tiles.append((code & 0xffff, code >> 16))
+    return tiles
+
+
+def check_grouped_whole(sizes, k, n, dtype, tiles, head=0, behind=0, odd=False):
+    from spi_amd.torch_utils.ops.grouped_linear import grouped_linear
+    g, offsets = gen(k + n), [head]
+    for s in sizes:
+        offsets.append(offsets[-1] + s)
+    t, e = offsets[-1] + behind, len(sizes)
+    place = lambda v: torch.cat([v.flatten()[:1], v.flatten()])[1:].view_as(v) if odd else v  # noqa: E731  (begins one value behind an aligned place)
+    x, w, dy = place(whole(g, t, k, dtype=dtype)), place(whole(g, e, n, k, dtype=dtype)), place(whole(g, t, n, dtype=dtype))
+    b, o = whole(g, e, n, dtype=dtype), torch.tensor(offsets, device=DEV, dtype=torch.int32)
+    assert grouped_tiles(x, w, dy, o) == tiles
+    leaves = [v.requires_grad_() for v in (x, w, b)]
+    y = grouped_linear(*leaves[:2], o, bias=b, gain=0.5)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    covered = torch.zeros(t, 1, device=DEV, dtype=torch.bool)
+    covered[head:offsets[-1]] = True
+    for v in (y, dx):
+        assert not v[:head].any() and not v[offsets[-1]:].any()
+    for i in range(e):
+        s = slice(offsets[i], offsets[i + 1])
+        xs, ws, ds = x[s].detach().double(), w[i].detach().double(), dy[s].double()
+        for name, got, exact in (('y', y[s], 0.5 * (xs @ ws.t()) + b[i].detach().double()), ('dx', dx[s], 0.5 * (ds @ ws)), ('dw', dw[i], 0.5 * (ds.t() @ xs)), ('db', db[i], ds.sum(0))):
+            same = got == exact.to(dtype)
+            assert same.all(), f'{name} of group {i}: {(~same).sum().item()} values, the first at {(~same).nonzero()[0].tolist()}'
+
+
+@pytest.mark.parametrize('dtype', [F32, F16, BF16])
+@pytest.mark.parametrize('sizes,k,n,tiles,kw', [
+    ([70, 0, 131], 136, 264, [(64, COPY)] * 3, {}),
+    ([70, 0, 131], 137, 263, [(64, WIDE)] * 3, {}),
+    ([2, 0, 1], 1, 1, [(64, EACH)] * 3, {}),
+    ([1311, 789], 2056, 2040, [(128, COPY)] * 3, {}),
+    ([1, 1408, 640], 2048, 2176, [(128, COPY)] * 3, dict(head=5, behind=140)),
+    ([1500, 1501], 2045, 2047, [(128, WIDE)] * 3, {}),
+    ([2999, 1], 2048, 2056, [(128, WIDE)] * 3, dict(head=1, odd=True)),                            # rows of whole 16 bytes on odd places
+    ([2001, 0, 2999], 3320, 3320, [(256, COPY)] * 3, {}),                                          # 260 tiles a pass: the last four cut into quarters
+    ([3000, 4000], 3320, 3320, [(256, COPY)] * 3, {}),                                             # 364 tiles, 108 of them cut; the weight gradient 338, 82 cut
+    ([4000, 0, 4000], 3312, 3320, [(256, COPY)] * 3, dict(head=300, behind=1)),                    # 34 x 13 = 442 tiles, none cut
+    ([256] * 16 + [512], 4096, 4096, [(256, COPY)] * 3, {}),                                       # tiles without an edge
+], ids=lambda v: None if not isinstance(v, list) else '-'.join(map(str, v)) if not isinstance(v[0], tuple) else f'{v[0][0]}')
+def test_grouped_tiles(sizes, k, n, tiles, kw, dtype):
+    check_grouped_whole(sizes, k, n, dtype, tiles, **kw)
+
+
+@pytest.mark.parametrize('m,n,k,padded,tiles', [
+    # (edge, loader) of int8 rows that begin on 16 bytes if `padded`, and of rows of floats, which the call lays out on 16 bytes
+    (100, 333, 1040, True, [(64, COPY), (64, COPY)]), (100, 333, 1031, True, [(64, WIDE), (64, COPY)]), (100, 333, 1031, False, [(64, WIDE), (64, WIDE)]),
+    (17, 1, 3, False, [(64, EACH), (64, EACH)]), (2100, 2090, 1040, True, [(128, COPY), (128, COPY)]), (2100, 2090, 1031, True, [(64, WIDE), (128, COPY)]),
+    (2600, 2500, 1031, True, [(128, WIDE), (128, COPY)]), (2600, 2500, 1031, False, [(128, WIDE), (128, WIDE)]), (4100, 4000, 1040, True, [(256, COPY), (256, COPY)]),
+    (4100, 4003, 1031, True, [(128, WIDE), (256, COPY)]), (4096, 4352, 2048, True, [(256, COPY), (256, COPY)])])
+def test_linear_int8_tiles(m, n, k, padded, tiles):
+    from spi_amd import hip
+    from spi_amd.torch_utils.ops.linear_int8 import linear_int8
+    g, pitch = gen(m + n + k), (k + 15) // 16 * 16 if padded else k
+
+    def rows(count):                                                  # what stands behind a row is not 0
+        full = torch.full((count, pitch), 99, device=DEV, dtype=torch.int8)
+        full[:, :k] = whole(g, count, k, dtype=torch.int8, most=127)
+        full[:, 0] = 127                                              # so that rows of floats have the scale 1, and quantise to themselves
+        return full[:, :k]
+    q, w, one = rows(m), rows(n), torch.ones(max(m, n), device=DEV)
+    exact = (q.double() @ w.double().t()).float()                     # integers: exact in 64 bits, rounded once
+    for x, scale, tile in zip((q, q.float()), (one[:m], None), tiles):
+        d = hip.LinearInt8Desc(m, n, k, hip.DTYPE_I8 if scale is not None else 0, 0, x.stride(0), w.stride(0), w.untyped_storage().nbytes(), x.data_ptr(), one.data_ptr(), w.data_ptr(),
+                               one.data_ptr(), None, one.data_ptr(), 1, 0.0, 1.0, -1.0)
+        code = hip.lib().spi_linear_int8_tile(ctypes.byref(d))
+        assert (code & 0xffff, code >> 16) == tile
+        for dtype in (F32, BF16):
+            same = linear_int8(x, w, one[:n], x_scale=scale, out_dtype=dtype) == exact.to(dtype)
+            assert same.all(), f'{(~same).sum().item()} values, the first at {(~same).nonzero()[0].tolist()}'
