@@ -257,3 +257,48 @@ def test_linear_int8_tiles(m, n, k, padded, tiles):
         for dtype in (F32, BF16):
             same = linear_int8(x, w, one[:n], x_scale=scale, out_dtype=dtype) == exact.to(dtype)
             assert same.all(), f'{(~same).sum().item()} values, the first at {(~same).nonzero()[0].tolist()}'
+
+
+# ---- a block in 8 bits against the block in floats -----------------------------------------------------------------------------------------
+def test_block_in_8_bits_is_the_float_block_within_its_roundings():
+    """norm -> 8-bit layer -> 8-bit layer -> norm and residual, against the same block in 64 bits with the weights as they were.
+
+    The four roundings to 8 bits (of both layers' rows and weights) are at most half a step each and independent: uniform, of variance step^2 / 12.  A product's error is a sum of 512
+    or 1024 of them with known factors, so its deviation follows; an activation of slope <= 1 does not widen it, and eight deviations are asked for (one value in 1e15 lies outside).
+    The rounding of the hidden rows to their type adds half a step, u |hidden|.  Through the norm, x -> x / sigma(x): |d| / sigma + |x| |1/sigma' - 1/sigma|, and sigma, a root mean square,
+    moves by at most the root mean square of d (allowed here: twice its deviation)."""
+    from spi_amd.torch_utils.ops.linear_int8 import linear_int8, quantize_rows
+    from spi_amd.torch_utils.ops.norm_residual import norm_residual
+    g = gen(40)
+    for rows, dtype in ((1, F32), (14, BF16), (200, F16)):
+        i = norm_inputs((rows, 512), dtype, 'rms', 'both', 'channel', False, seed=rows)
+        w1, w2 = randn(g, 1024, 512), randn(g, 512, 1024)
+        (q1, s1), (q2, s2) = quantize_rows(w1), quantize_rows(w2)
+        stream, (q, qs) = norm_residual(i['h'], i['residual'], gate=i['gate'], scale=0.1, post_weight=i['post_weight'], pre_weight=i['pre_weight'], eps=1e-6, quantize=True)
+        hidden = linear_int8(q, q1, s1, x_scale=qs, act='lrelu', gain=512 ** -0.5, out_dtype=dtype)
+        y2 = linear_int8(hidden, q2, s2)
+        out, _ = norm_residual(y2, stream, scale=0.1, post_weight=i['post_weight'], where='after', eps=1e-6)
+        # the float block
+        s64, y64 = norm_case(i, 0.1, 'rms', 'both', 1e-6, 'linear', fn=ref.norm_residual)
+        w1, w2, u = w1.double(), w2.double(), ref.half_step(dtype)
+        h64 = ref.activation('lrelu', y64 @ w1.t()) * 512 ** -0.5
+        x64 = h64 @ w2.t()
+        sigma = torch.sqrt((x64 ** 2).mean(-1, keepdim=True) + 1e-6)
+        o64 = s64 + 0.1 * x64 / sigma * i['post_weight'].double()
+
+        def variance(step, q, s, x, before):                          # of a product's error: (step^2 / 12 + before) through the weights, and the weights' own roundings
+            w = q.double() * s.double()[:, None]
+            return (step ** 2 / 12 + before) @ (w ** 2).t() + s.double() ** 2 / 12 * (x ** 2).sum(-1, keepdim=True)
+        one = torch.ones_like(y64)
+        v1 = variance(qs.double()[:, None] * one, q1, s1, y64, 0 * one) / 512
+        t2 = hidden.double().abs().amax(-1, keepdim=True) / 127
+        v2 = variance(t2 * torch.ones_like(h64), q2, s2, h64, v1 + (u * h64) ** 2) + (u * x64) ** 2
+        d, moved = 8 * v2.sqrt(), 2 * v2.mean(-1, keepdim=True).sqrt()
+        through = (d + (x64.abs() + d) * moved / (sigma - moved)) / sigma * i['post_weight'].double().abs()
+        bound = 0.1 * through + 2 * u * (s64.abs() + o64.abs()) + piled(512) * ref.U32 * o64.abs()
+        worst = ((out.double() - o64).abs() / bound).max().item()
+        assert worst <= 1, (rows, dtype, worst)
+        # The bound means something, about a fifth of the 0.1 that the block adds to a value: with the largest of a row at four deviations, a rounding is 4 / 127 / 12^0.5 = 0.0091 of the
+        # rows (0.0126 of the hidden ones, whose root mean square the activation takes to 0.72), 0.0091 of either weight; with bf16's two of 2^-8, 0.021 together.  Eight of it, and
+        # twice of it times 0.8 + 8 * 0.021 for the deviation that divides, over 1 - 2 * 0.021: 0.218.
+        assert (0.1 * through).mean() < 0.022
