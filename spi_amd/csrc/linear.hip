@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) int8_tile_kernel(cons
 
 // Up to 16 rows: 16 outputs a block, the summed axis over its four waves, whose weights go straight from memory to the matrix cores (v_mfma_i32_16x16x64_i8) -- all of a wave's
 // loads under way at once.  The rows wait in LDS: int8 rows as they are; up to four rows of floats are quantised by every block, each for itself (one launch fewer).
-// Bound by latency: 1 x 512 x 512 4.0 us (as a tile of 64 x 64 behind a launch that quantises: 5.2 + 2.1), 14 x 2048 x 4096 (8 MB of weights) 6.3 us (9.1).
+// Bound by latency: 1 x 512 x 512 4.3 us (as a tile of 64 x 64 behind a launch that quantises: 5.2 + 2.1), 14 x 2048 x 4096 (8 MB of weights) 6.4 us (9.1).
 constexpr int FEW = 16, FEW_FLOATS = 4, FEW_LDS = 60000;
 __host__ __device__ inline int few_pitch(int K) { return (K + 63) / 64 * 64 + 16; }
 
@@ -421,7 +421,7 @@ __global__ void __launch_bounds__(SIZE == 256 ? 512 : 256) grouped_tile_kernel(c
     grouped_tile<E, T, PASS>(a, t, r0, c0, s0, s1);
 }
 // db[e][n] = sum of dy over the group's rows, in two steps of a fixed order: part s of S of the group's rows into part [E][S][N] (S = 1: straight into db), then the
-// parts.  A block takes 64 chunks of VEC columns by four rows at a time.  Bound by HBM: 16384 x 2048 bf16 12.8 us = 5.2 TB/s, and 4.8 us for the parts.
+// parts.  A block takes 64 chunks of VEC columns by four rows at a time.  Bound by HBM: 16384 x 2048 bf16 12.8 us = 5.2 TB/s, and 5.2 us for the parts.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) grouped_bias_grad_kernel(const GroupArgs a, float* __restrict__ part, int S) {
     __shared__ float sum[4][64][VEC + 1];
@@ -476,9 +476,12 @@ void bias_grad(const spi_grouped_linear_desc& d, const GroupArgs& a, hipStream_t
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // Edge of the tiles, from the number of tiles that there would be (`rows`(edge) tile rows).  A tile of 256 reads a fourth of what sixteen of 64 do, but a chip half idle costs
-// more.  Measured, bf16 forward, edges 64 / 128 / 256: 2048 x 1024 x 1024 in 4 groups (144 tiles of 128) 11.4 / 15.8 / 15.5 us, 8192 x 1024 x 1024 in 8 (544, 128 of 256)
-// 32.5 / 25.2 / 31.6, 16384 x 2048 x 2048 in 8 (512 of 256) 307 / 206 / 196; int8 4096^3 (256 of 256) 130 / 105 / 94.  Through registers (rows on odd places) 128 pays later:
-// bf16 weight gradient of 8192 x 1003 x 501 (256 tiles of 128) 37 / 55.
+// more.  Measured, edges 64 / 128 / 256, us: bf16 forward 2048 x 1024 -> 1024 in 4 groups (144 tiles of 128) 11.5 / 15.6 / 17.0, 8192 x 1024 -> 1024 in 8 (544, 128 of 256)
+// 33 / 25 / 34, 16384 x 2048 -> 2048 in 8 (512 of 256) 212 / 147 / 130; int8 4096 x 4096 -> 4096 (256 of 256) 127 / 105 / 95.  Rows that pass through registers pay for 128 later:
+// fp32 4099 x 515 -> 771 in 5, weight gradient (175 tiles of 128) 74 / 134, row gradient (170) 58 / 74; bf16 8192 x 1003 -> 501 in 8, forward (272) 29 / 31, weights (256) 31 / 29,
+// rows (544) 32 / 25.
+// The rule counts tiles, not how full they are: 8192 x 1024 -> 2048 in 24 ragged groups, whose tiles of 256 are a fourth padding, takes 82 us from memory where tiles of 128 take 75
+// (from the cache 59 and 62).
 struct Tile { int edge, load; };
 // rows(edge): tile rows at that edge; smallest: bytes of the smaller operand, from its first value to its tensor's end.  Rows that cannot be copied to LDS as they lie are read 16
 // bytes at a time, which takes operands of 16 bytes at least -- whatever the edge, and for a sum over nothing, too: the first step's loads come before the count of steps.

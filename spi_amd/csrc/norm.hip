@@ -4,7 +4,7 @@
 //   s = residual + scale * a(gate) * z      (the residual stream, rounded once to the row type)
 //   y = Norm(s) * pre_weight + pre_bias     (for the next block; from the UNROUNDED s), or its rows in 8 bits
 //
-// Bound by HBM: h and residual in, s and y out, once each (4 x 4096 x 2048 bf16: 72 us = 3.7 TB/s, where a copy of 1 GiB reaches 5.1).  A row stays in the
+// Bound by HBM: h and residual in, s and y out, once each (4 x 4096 x 2048 bf16: 74 us = 3.6 TB/s, where a copy of 1 GiB reaches 5.2).  A row stays in the
 // registers of the threads that loaded it, so both norms' sums run over registers; sums are fp32 (a row whose squares pass the fp32 range has a deviation of
 // infinity, and is normalised to 0).
 #include "typed.hpp"
@@ -227,8 +227,8 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float* red, int& ph
 }
 
 // Bound by HBM (h, residual, ds, dy in; d_h, d_residual out) as far as enough of it is under way: a block holds few rows, so the next row's values are on their way while a
-// row is worked on, in loads without a condition (a load under one is waited for at once).  4 x 4096 x 2048 bf16: 105 us = 3.8 TB/s; 139 us with conditional loads, with or
-// without the sums between the threads; 184 us without the next row.
+// row is worked on, in loads without a condition (a load under one is waited for at once).  4 x 4096 x 2048 bf16: 109 us = 3.7 TB/s.  (When it was
+// chosen, on one card: 105; 139 with conditional loads, with or without the sums between the threads; 184 without the next row.)
 template <typename T, int VEC, int TPR, int NV, bool LAYER>
 __global__ void __launch_bounds__(TPR > BT ? TPR : BT, TPR > BT ? 4 : sizeof(T) == 4 && NV == 1 ? 3 : 2) norm_bwd_kernel(const NormBwdArgs a) {
     constexpr int G = TPR > BT ? 1 : BT / TPR;

@@ -44,8 +44,8 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
 // One operand of a tile.  p: its first value; pitch: bytes between neighbours on the axis that is not adjacent; k: values of the summed axis; n: valid values of the
 // tile's own axis; bytes: what may be read from p on (row: n * pitch; col: k * pitch less the bytes of a row before p).  256 * pitch < 2^31.
-// Summed values behind k are 0 in the tile; so are rows behind n of a `row` operand.  Columns behind n of a `col` operand may hold what follows in memory: they only reach
-// results that lie outside, too.  end: bytes from p to the end of the tensor that the operand is part of.
+// Summed values behind k are 0 in the tile.  Rows (`row`) or columns (`col`) behind n may hold what follows in memory, or 0: they only reach results that lie outside, too.
+// end: bytes from p to the end of the tensor that the operand is part of.
 struct TileOperand { const char* p; int64_t pitch, bytes, k; int n; int64_t end; };
 
 // row: which chunk a tile row's chunks are XORed with, so that 16 rows' chunks c fall on all of the 64 banks (and eight rows' on 32)
@@ -188,8 +188,8 @@ struct TileReader {
     }
 };
 
-// Two stages of LDS: the copies of step k + 1 are under way while step k is multiplied, one barrier a step.  (Four stages, and steps of 64 bytes, were measured slower:
-// 16384 x 2048 x 2048 bf16 at 256 x 256, 143 us against 132: half cache lines, and the latency is already covered.)
+// Two stages of LDS: the copies of step k + 1 are under way while step k is multiplied, one barrier a step.  (16384 x 2048 x 2048 bf16 at 256 x 256, both sides on one card: 132 us; four
+// stages of 64 bytes of the summed axis, 143: half cache lines, and the latency is already covered.)
 template <typename T, int BM_, int BN_, int GM_, int GN_, bool COLA, bool COLB, int LOAD>
 struct TileEngine {
     static constexpr int BM = BM_, BN = BN_, GM = GM_, GN = GN_, NW = GM * GN, WM = BM / GM, WN = BN / GN, FM = WM / 32, FN = WN / 32, KT = 128 / (int)sizeof(T),

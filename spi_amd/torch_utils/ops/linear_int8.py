@@ -53,7 +53,8 @@ def linear_int8(x, weight_q, weight_scale, bias=None, x_scale=None, act='linear'
     """x [..., K] -> y [..., N].
 
     x             fp32 / fp16 / bf16 rows, quantised by the call as ``quantize_rows`` does, or int8 rows with their ``x_scale`` [...] (fp32)
-    weight_q      int8 [N, K] and weight_scale fp32 [N], from ``quantize_rows(weight)``; rows that do not begin on 16 bytes are copied by every call
+    weight_q      int8 [N, K] and weight_scale fp32 [N], from ``quantize_rows(weight)``, whose rows begin on 16 bytes: fastest.  Rows of adjacent values at other places, at most
+                  2^22 bytes apart, are read as they lie; any others are copied by every call
     bias          [N] (fp32) or None;  act, alpha, gain, clamp as in ``bias_act``
     out_dtype     fp32 / fp16 / bf16; default: x's type, fp32 for int8 rows
 
